@@ -327,6 +327,21 @@ int64_t b200_client_launch_count(const b200_client* client);
 b200_error* b200_matmul_f32_static_scratch(const float* a, const float* b, float* c, int64_t m, int64_t n, int64_t k,
                                            void* cuda_stream);
 
+/* ---- moves inside a paged cache (no counterpart in the reference, whose example keeps one dense cache per layer,
+ *      examples/gemma/main.py:113-123). A cache is a buffer [layers, 2 (keys, values), pages, page size, key-value heads, features] of
+ *      f32, bf16 or f16 that lives across programs: a program reads it through `stablehlo.custom_call @b200.paged_attention`, and
+ *      these calls change it in place, in the order of the client's work (behind executions enqueued before, in front of those
+ *      enqueued after; pending reads to the host are waited for on the device). The indices are host memory and are read before the call returns. A
+ *      token's keys of one layer have to be a multiple of 16 bytes. ---- */
+/* Row i of `rows`, a buffer [layers, 2, num_slots, key-value heads, features] of the cache's type, goes to position
+ * slots[i] % page size of page slots[i] / page size in every layer; a negative slot leaves its row out (padding). Two rows for one
+ * slot and slots behind the cache are refused, and nothing is written then. */
+b200_error* b200_cache_write_pages(b200_client* client, b200_buffer* cache, b200_buffer* rows, const int32_t* slots, size_t num_slots);
+/* pairs[2 i] is the page that is copied, pairs[2 i + 1] the one that becomes its copy, in every layer. All sources are read as they
+ * were before the call, whatever the order of the pairs, so chains and exchanges are fine; two pairs for one destination and pages
+ * outside the cache are refused, and nothing is written then. */
+b200_error* b200_cache_copy_pages(b200_client* client, b200_buffer* cache, const int32_t* pairs, size_t num_pairs);
+
 #pragma GCC visibility pop
 #ifdef __cplusplus
 }

@@ -166,6 +166,8 @@ SIGNATURES = {
     "b200_profiler_destroy": (_P, [_P]),
     "b200_client_set_profiling": (_P, [_P, C.c_int]),
     "b200_client_profile_report": (_P, [_P, C.POINTER(_P)]),
+    "b200_cache_write_pages": (_P, [_P, _P, _P, _P, C.c_size_t]),
+    "b200_cache_copy_pages": (_P, [_P, _P, _P, C.c_size_t]),
     "b200_matmul_f32_static_scratch": (_P, [_P, _P, _P, C.c_int64, C.c_int64, C.c_int64, _P]),
 }
 
@@ -615,10 +617,39 @@ class Client:
         _check(load_library().b200_matmul_f32_static_scratch(a.device_pointer(), b.device_pointer(),
                                                              out.device_pointer(), m, n, k, self.compute_stream()))
 
+    def write_pages(self, cache: Buffer, rows: Buffer, slots):
+        """Rows [layers, 2, n, kv_heads, head_dim] of n tokens into a cache [layers, 2, pages, page_size, kv_heads, head_dim], in
+        place: row i goes to position slots[i] % page_size of page slots[i] // page_size (`slots`: whole numbers on the host; a
+        negative one leaves its row out). Enqueued in the order of the client's work; slots are distinct."""
+        index = _indices(slots, 1)
+        _check(_lib.b200_cache_write_pages(self._h, cache._h, rows._h, index.ctypes.data, len(index)))
+
+    def copy_pages(self, cache: Buffer, pairs):
+        """Page pairs[i][0] of a cache onto page pairs[i][1], keys and values of all layers, in place. Every source is read as it
+        was before the call; destinations are distinct."""
+        index = _indices(pairs, 2)
+        _check(_lib.b200_cache_copy_pages(self._h, cache._h, index.ctypes.data, len(index)))
+
     def close(self):
         if getattr(self, "_h", None) and self._owned:
             load_library().b200_client_destroy(self._h)
             self._h = None
+
+
+def _indices(values, ndim: int) -> np.ndarray:
+    """Indices on the host as the library reads them: [n], or [n, 2] for pairs."""
+    if type(values) is np.ndarray and values.dtype == np.int32 and values.flags.c_contiguous:
+        a = values
+    else:
+        a = np.asarray(values)
+        if a.size and (a.dtype.kind not in "iu" or a.min() < -2**31 or a.max() >= 2**31):
+            raise B200Error("slots and pages have to be whole numbers of 32 bits", INVALID_ARGUMENT)
+        a = np.ascontiguousarray(a, np.int32)
+    if a.size == 0:
+        a = a.reshape((0,) if ndim == 1 else (0, 2))
+    if a.ndim != ndim or (ndim == 2 and a.shape[1] != 2):
+        raise B200Error("slots have to be one list of numbers" if ndim == 1 else "pages have to be a list of pairs", INVALID_ARGUMENT)
+    return a
 
 
 class DeviceGroup:

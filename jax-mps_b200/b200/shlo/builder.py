@@ -827,6 +827,50 @@ class Builder:
         props.update(attrs or {})
         return self.emit("stablehlo.custom_call", list(xs), list(result_types), props=props)
 
+    # ---- operators of large language models (custom calls @b200.*) ---------------
+    def _operator(self, name: str, xs: Sequence[Val], result_types, config: dict) -> list[Val]:
+        """A custom call @b200.<name>; the attributes that are given stand in its backend_config dictionary."""
+        text = ", ".join(f"{k} = {v:.9e} : f32" if isinstance(v, float) else f"{k} = {int(v)} : i64" for k, v in config.items() if v is not None)
+        return list(self.custom_call(f"b200.{name}", xs, result_types, attrs={"api_version": "4 : i32", "backend_config": "{" + text + "}"}))
+
+    def paged_attention(self, q: Val, cache: Val, table: Val, lengths: Val, new: Val | None = None, *, layer: int = 0,
+                        scale: float | None = None, window: int = 0, sinks: int = 0) -> Val:
+        """Attention of one new token per sequence over a cache of pages: q [batch, heads, head_dim], `cache` [layers, 2 (keys,
+        values), pages, page_size, kv_heads, head_dim] of which layer `layer` is read, `table` i32[batch, pages of a sequence] names
+        the pages of each sequence in order, `lengths` i32[batch] how many positions of them are filled. Query head h reads
+        key-value head h // (heads / kv_heads). `new` [2, batch, kv_heads, head_dim] is the token's own key and value, which are not in
+        the cache yet: the token stands at position lengths[b] then, otherwise at lengths[b] - 1, the last cached one. With a
+        `window`, position j is visible from p when p - j < window or j < sinks. `scale` is 1 / sqrt(head_dim) by default. A
+        sequence that sees nothing gives zeros; lengths below zero count as zero and above the table's room as that; pages
+        that the table names outside the cache are left out. f32, bf16 or f16, sums in 32 bits. No gradient."""
+        xs = [q, cache, table, lengths] + ([new] if new is not None else [])
+        config = {"layer": layer, "scale": None if scale is None else float(scale), "window": window, "sinks": sinks}
+        return self._operator("paged_attention", xs, [(q.shape, q.dtype)], config)[0]
+
+    def window_attention(self, q: Val, k: Val, v: Val, lengths: Val | None = None, *, scale: float | None = None, window: int = 0,
+                         sinks: int = 0) -> Val:
+        """Causal attention of whole prompts: q [batch, tokens, heads, head_dim], k and v [batch, tokens, kv_heads, head_dim], and for
+        a padded batch `lengths` i32[batch]; rows from a sequence's length on are zero and nobody sees them. `window`, `sinks` and
+        `scale` as in paged_attention. No gradient."""
+        xs = [q, k, v] + ([lengths] if lengths is not None else [])
+        config = {"scale": None if scale is None else float(scale), "window": window, "sinks": sinks}
+        return self._operator("window_attention", xs, [(q.shape, q.dtype)], config)[0]
+
+    def token_log_probs(self, logits: Val, tokens: Val, top: int = 0) -> list[Val]:
+        """For logits [rows, vocab] (f32, bf16, f16) and tokens i32[rows]: the tokens' log probabilities (0 for a token outside the
+        vocabulary, which is how padding is named), the entropies and the logarithms of the normalisers, f32[rows] each; with
+        `top` also the log probabilities f32[rows, top] and numbers i32[rows, top] of the most probable tokens (equal
+        logits by their number, at most 128). Differentiable in the logits through the first three."""
+        rows = logits.shape[0]
+        types = [((rows,), "f32")] * 4 + ([((rows, top), "f32"), ((rows, top), "i32")] if top else [])
+        # the fourth is what the normaliser loses to its rounding
+        log_prob, entropy, norm, rest, *best = self._operator("token_log_probs", [logits, tokens], types, {"top": top} if top else {})
+
+        def vjp(g):
+            return [self._operator("token_log_probs_grad", [logits, tokens, norm, rest, entropy, *g], [(logits.shape, logits.dtype)], {})[0], None]
+        self.record([log_prob, entropy, norm], [logits, tokens], vjp)
+        return [log_prob, entropy, norm, *best]
+
     def optimization_barrier(self, xs: Sequence[Val]) -> list[Val]:
         xs = list(xs)
         return self.emit("stablehlo.optimization_barrier", xs, [(x.shape, x.dtype) for x in xs])

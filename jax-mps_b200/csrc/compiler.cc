@@ -142,6 +142,42 @@ bool few_of_many(const TensorType& t, int64_t k) {
 // ---------------------------------------------------------------------------
 // pass 1: inlining and pass-through removal
 // ---------------------------------------------------------------------------
+// The operators that a program reaches as custom calls.
+bool is_operator(const std::string& name) {
+  return name == "b200.paged_attention" || name == "b200.window_attention" || name == "b200.token_log_probs" || name == "b200.token_log_probs_grad";
+}
+
+// Attributes of a custom call: what stands in its `backend_config` (or `mhlo.backend_config`) dictionary.
+std::map<std::string, std::string> custom_call_config(const Op& op) {
+  std::map<std::string, std::string> out;
+  for (const char* key : {"backend_config", "mhlo.backend_config"}) {
+    if (!op.has(key)) continue;
+    const std::string& raw = op.attr(key);
+    size_t i = raw.find_first_not_of(" \t\n");
+    if (i == std::string::npos || raw[i] != '{') continue;               // the string form says nothing here
+    const size_t end = raw.rfind('}');
+    if (end == std::string::npos || end < i) throw CompileError("custom_call: unreadable backend_config " + raw);
+    i++;
+    while (i < end) {
+      size_t comma = raw.find(',', i);
+      if (comma == std::string::npos || comma > end) comma = end;
+      const std::string item = raw.substr(i, comma - i);
+      i = comma + 1;
+      const size_t eq = item.find('=');
+      auto trimmed = [](const std::string& s) {
+        const size_t a = s.find_first_not_of(" \t\n"), z = s.find_last_not_of(" \t\n");
+        return a == std::string::npos ? std::string() : s.substr(a, z - a + 1);
+      };
+      if (eq == std::string::npos) {
+        if (!trimmed(item).empty()) throw CompileError("custom_call: unreadable backend_config " + raw);
+        continue;
+      }
+      out[trimmed(item.substr(0, eq))] = trimmed(item.substr(eq + 1));
+    }
+  }
+  return out;
+}
+
 struct Inliner {
   Module& m;
   std::map<Value*, Value*> remap;
@@ -273,6 +309,16 @@ struct Inliner {
           return;
         }
       }
+      // Operators of large language models: the operation by its own name, checked and lowered by Planner::lower_operator. Any
+      // other target of this name space stays a custom_call and is refused as one.
+      if (is_operator(tgt)) {
+        auto config = custom_call_config(*op);
+        op->name = tgt;
+        op->attrs = std::move(config);
+        process(std::move(op), b);
+        return;
+      }
+      if (tgt.rfind("b200.", 0) == 0) throw CompileError("custom_call @" + tgt + " is not an operator of the B200 plugin");
     }
     // convert(convert(x, wider type), type of x) -> x when the first conversion is exact (bf16 -> f32 -> bf16 between two
     // products of a bf16 network)
@@ -1239,12 +1285,13 @@ struct DecodeAttentionFusion {
 // ---------------------------------------------------------------------------
 // op classification
 // ---------------------------------------------------------------------------
-enum class Cat { ELEMENTWISE, DUP, INDEXING, REDUCE, DOT, CONV, SCATTER, WINDOW, SORT, RNG, LINALG, ATTENTION, WHILE, CASE, ALL_REDUCE, ALL_GATHER, RETURN, TOKEN, PARTITION_ID, UNSUPPORTED };
+enum class Cat { ELEMENTWISE, DUP, INDEXING, REDUCE, DOT, CONV, SCATTER, WINDOW, SORT, RNG, LINALG, ATTENTION, OPERATOR, WHILE, CASE, ALL_REDUCE, ALL_GATHER, RETURN, TOKEN, PARTITION_ID, UNSUPPORTED };
 
 Cat categorize(Op* op) {
   const std::string sh = op->short_name();
   if (sh == "return") return Cat::RETURN;
   if (op->name == "b200.decode_attention") return Cat::ATTENTION;
+  if (is_operator(op->name)) return Cat::OPERATOR;
   if (op->name.rfind("stablehlo.", 0) != 0 && op->name.rfind("chlo.", 0) != 0 && op->name.rfind("mhlo.", 0) != 0)
     return Cat::UNSUPPORTED;
   if (is_elementwise_op(sh)) return Cat::ELEMENTWISE;
@@ -2819,6 +2866,147 @@ struct Planner {
     s.block[0] = 256; s.block[1] = s.block[2] = 1;
     s.args = {slot_of.at(out), parts};
     s.n_outs = 1;
+    plan.steps.push_back(std::move(s));
+  }
+
+  // Operators that programs name as custom calls (operators.h): operand and attribute checks, the launch description, scratch.
+  void lower_operator(Op* op, Plan& plan, BlockState& st) {
+    auto fail = [&](const std::string& why) { throw CompileError(op->name + ": " + why); };
+    std::set<std::string> known;
+    auto number = [&](const char* name, double otherwise) {
+      known.insert(name);
+      if (!op->has(name)) return otherwise;
+      const std::string& raw = op->attr(name);
+      char* end = nullptr;
+      const double v = strtod(raw.c_str(), &end);
+      if (end == raw.c_str() || !std::isfinite(v)) fail(std::string("attribute ") + name + " is no number: " + raw);
+      return v;
+    };
+    auto whole = [&](const char* name, long long otherwise, long long lo, long long hi) {
+      const double v = number(name, (double)otherwise);
+      if (v != std::floor(v) || v < (double)lo || v > (double)hi)
+        fail(std::string("attribute ") + name + " has to be a whole number from " + std::to_string(lo) + " to " + std::to_string(hi) + ", got " + op->attr(name));
+      return (long long)v;
+    };
+    const auto& in = op->operands;
+    const auto& out = op->results;
+    auto want = [&](Value* v, const char* what, DT dt, const std::vector<int64_t>& dims) {
+      TensorType t;
+      t.dt = dt;
+      t.dims = dims;
+      if (!(v->type == t)) fail(std::string(what) + " has to be " + t.str() + ", got " + v->type.str());
+    };
+    auto count = [&](size_t least, size_t most, size_t results) {
+      if (in.size() < least || in.size() > most || out.size() != results)
+        fail("takes " + std::to_string(least) + (most > least ? " to " + std::to_string(most) : "") + " operands and gives " + std::to_string(results) + " results, got " +
+             std::to_string(in.size()) + " and " + std::to_string(out.size()));
+    };
+    auto type_of = [&](Value* v, const char* what) {
+      const DT dt = v->type.dt;
+      if (dt != DT::F32 && dt != DT::BF16 && dt != DT::F16) fail(std::string(what) + " has to be f32, bf16 or f16, got " + v->type.str());
+      return dt == DT::F32 ? 0 : dt == DT::BF16 ? 1 : 2;
+    };
+    auto rank = [&](Value* v, const char* what, int r) {
+      if (v->type.rank() != r) fail(std::string(what) + " has to have " + std::to_string(r) + " dimensions, got " + v->type.str());
+    };
+    auto fits = [&](int64_t n, const char* what) {
+      if (n < 0 || n >= (1LL << 31)) fail(std::string(what) + " of 2^31 and more");
+      return (int)n;
+    };
+    OperatorLaunch o;
+    auto heads = [&](int64_t h, int64_t kv, int64_t d) {
+      o.heads = fits(h, "heads"), o.kv_heads = fits(kv, "key-value heads"), o.dim = fits(d, "head features");
+      if (h < 1 || kv < 1 || h % kv) fail("the number of query heads (" + std::to_string(h) + ") has to be a multiple of the number of key-value heads (" + std::to_string(kv) + ")");
+      if (d < 8 || d > 256 || d % 8) fail("head features have to be a multiple of 8 from 8 to 256, got " + std::to_string(d));
+      o.scale = (float)number("scale", 1.0 / std::sqrt((double)d));
+      o.window = (int)whole("window", 0, 0, (1LL << 30));
+      o.sinks = (int)whole("sinks", 0, 0, (1LL << 30));
+      if (o.sinks && !o.window) fail("sinks without a window");
+    };
+    if (op->name == "b200.paged_attention") {
+      count(4, 5, 1);
+      o.kind = OperatorLaunch::PAGED_ATTENTION;
+      Value *q = in[0], *cache = in[1], *table = in[2];
+      o.type = type_of(q, "q");
+      rank(q, "q", 3);
+      rank(cache, "the cache", 6);
+      rank(table, "the page table", 2);
+      const auto& qd = q->type.dims;
+      const auto& cd = cache->type.dims;
+      heads(qd[1], cd[4], qd[2]);
+      o.batch = fits(qd[0], "batch");
+      o.pages = fits(cd[2], "pages"), o.page = fits(cd[3], "page size"), o.width = fits(table->type.dims[1], "pages of a sequence");
+      if (cd[3] < 1) fail("a page holds one position at least");
+      o.layer = (int)whole("layer", 0, 0, std::max<int64_t>(cd[0] - 1, 0));
+      want(cache, "the cache [layers, 2, pages, page size, key-value heads, features]", q->type.dt, {cd[0], 2, cd[2], cd[3], cd[4], qd[2]});
+      if (cd[0] < 1) fail("the cache has no layer");
+      want(table, "the page table", DT::I32, {qd[0], table->type.dims[1]});
+      want(in[3], "the lengths", DT::I32, {qd[0]});
+      o.has_new = in.size() > 4;
+      if (o.has_new) want(in[4], "the new keys and values", q->type.dt, {2, qd[0], cd[4], qd[2]});
+      want(out[0], "the result", q->type.dt, qd);
+    } else if (op->name == "b200.window_attention") {
+      count(3, 4, 1);
+      o.kind = OperatorLaunch::WINDOW_ATTENTION;
+      Value *q = in[0], *k = in[1];
+      o.type = type_of(q, "q");
+      rank(q, "q", 4);
+      rank(k, "k", 4);
+      const auto& qd = q->type.dims;
+      heads(qd[2], k->type.dims[2], qd[3]);
+      o.batch = fits(qd[0], "batch"), o.tokens = fits(qd[1], "tokens");
+      const std::vector<int64_t> kd = {qd[0], qd[1], k->type.dims[2], qd[3]};
+      want(k, "k", q->type.dt, kd);
+      want(in[2], "v", q->type.dt, kd);
+      o.has_lengths = in.size() > 3;
+      if (o.has_lengths) want(in[3], "the lengths", DT::I32, {qd[0]});
+      want(out[0], "the result", q->type.dt, qd);
+    } else {
+      const bool grad = op->name == "b200.token_log_probs_grad";
+      o.kind = grad ? OperatorLaunch::TOKEN_LOG_PROBS_GRAD : OperatorLaunch::TOKEN_LOG_PROBS;
+      o.top = grad ? 0 : (int)whole("top", 0, 0, 128);
+      count(grad ? 8 : 2, grad ? 8 : 2, grad ? 1 : o.top ? 6 : 4);
+      o.type = type_of(in[0], "the logits");
+      rank(in[0], "the logits", 2);
+      o.rows = in[0]->type.dims[0];
+      o.vocab = fits(in[0]->type.dims[1], "vocabulary");
+      if (o.vocab < 1) fail("the vocabulary is empty");
+      if (o.top > o.vocab) fail("more alternatives (" + std::to_string(o.top) + ") than the vocabulary has (" + std::to_string(o.vocab) + ")");
+      want(in[1], "the tokens", DT::I32, {o.rows});
+      if (grad) {
+        for (int k = 2; k < 8; k++) want(in[k], "an operand of the gradient", DT::F32, {o.rows});
+        want(out[0], "the result", in[0]->type.dt, in[0]->type.dims);
+      } else {
+        for (int k = 0; k < 4; k++) want(out[k], "a result", DT::F32, {o.rows});
+        if (o.top) {
+          want(out[4], "the alternatives' log probabilities", DT::F32, {o.rows, o.top});
+          want(out[5], "the alternatives", DT::I32, {o.rows, o.top});
+        }
+      }
+    }
+    for (auto& kv : op->attrs)
+      if (!known.count(kv.first)) fail("no attribute of this name: " + kv.first);
+    for (Value* v : out) ensure_slot(v, st);
+    if (out[0]->type.numel() == 0) return;
+    if (const char* why = operator_plan(o)) fail(why);
+    Step s;
+    s.kind = Step::OPERATOR;
+    s.label = op->name.substr(5);
+    for (auto& kv : op->attrs) s.label += " " + kv.first + "=" + kv.second.substr(0, kv.second.find(' '));
+    s.n_outs = (int)out.size();
+    for (Value* v : out) s.args.push_back(slot_of.at(v));
+    for (Value* v : in) {
+      if (!slot_of.count(v)) throw CompileError("internal: operand of " + op->name + " has no storage");
+      s.args.push_back(slot_of.at(v));
+    }
+    if (o.scratch_bytes > 0) {
+      TensorType t;
+      t.dt = DT::U8;
+      t.dims = {(int64_t)o.scratch_bytes};
+      s.args.push_back(new_slot(Slot::TEMP, t, st.arena));
+    }
+    if (o.waits) prog.tensor_saving = 1e30;
+    s.op = o;
     plan.steps.push_back(std::move(s));
   }
 
@@ -6170,6 +6358,10 @@ struct Planner {
           lower_decode_attention(op, plan, st);
           break;
         }
+        case Cat::OPERATOR: {
+          lower_operator(op, plan, st);
+          break;
+        }
         case Cat::LINALG: {
           if (op->short_name() == "cholesky") lower_cholesky(op, plan, st);
           else if (op->short_name() == "top_k") lower_top_k(op, plan, st);
@@ -6587,6 +6779,7 @@ void dump_plan(const CompiledProgram& prog, const Plan& p, std::ostringstream& o
         os << "transpose batch=" << s.iparams[1] << " rows=" << s.iparams[2] << " cols=" << s.iparams[3] << " bytes=" << s.iparams[0]
            << " dst_off=" << s.iparams[6];
         break;
+      case Step::OPERATOR: os << "operator " << s.label; break;
       case Step::REPACK16: os << "repack16 rows=" << s.iparams[0] << " cols=" << s.iparams[1] << " ld " << s.iparams[3] << "->" << s.iparams[2]; break;
       case Step::WHILE:
         os << "while trip=" << s.trip_count << " exchanged=" << std::count(s.swap.begin(), s.swap.end(), (char)1) << "/" << s.state.size();
@@ -6617,7 +6810,7 @@ uint64_t fnv1a(const std::string& s) {
 
 bool graph_safe_step(const Step& s) {
   switch (s.kind) {
-    case Step::KERNEL: case Step::IGEMM: case Step::MEMCPY: case Step::GEMM16: case Step::REPACK16: case Step::TRANSPOSE: case Step::SPLIT_B: return true;
+    case Step::KERNEL: case Step::IGEMM: case Step::MEMCPY: case Step::GEMM16: case Step::REPACK16: case Step::TRANSPOSE: case Step::SPLIT_B: case Step::OPERATOR: return true;
     case Step::WHILE: return s.trip_count >= 0 && graph_safe(*s.sub[1]);
     default: return false;
   }
@@ -6767,6 +6960,7 @@ std::unique_ptr<CompiledProgram> compile_module(Module& m, const CompileOptions&
         else if (s.kind == Step::GEMM16) n += (s.g16.path == 0 && s.g16.split_k > 1) ? 2 : 1;
         else if (s.kind == Step::REPACK16) n += (s.iparams[0] + 65534) / 65535;
         else if (s.kind == Step::TRANSPOSE) n += 1;
+        else if (s.kind == Step::OPERATOR) n += s.op.launches;
         else if (s.kind == Step::WHILE) {
           if (s.trip_count < 0) { dynamic = true; continue; }
           n += s.trip_count * count(*s.sub[1]);      // a counted loop never evaluates its condition

@@ -14,6 +14,7 @@
 
 #include "gemm16.h"
 #include "gemm32.h"
+#include "operators.h"
 #include "tile32.h"
 #include "ir.h"
 
@@ -67,7 +68,7 @@ long long scatter_elems_scratch_ints(long long updates);
 int scatter_elems_launches(long long numel);
 
 struct Step {
-  enum Kind { KERNEL, IGEMM, MEMCPY, MEMSET, WHILE, CASE, ALL_REDUCE, SCATTER, JOIN, GEMM16, REPACK16, TRANSPOSE, ALL_GATHER, SPLIT_B } kind = KERNEL;
+  enum Kind { KERNEL, IGEMM, MEMCPY, MEMSET, WHILE, CASE, ALL_REDUCE, SCATTER, JOIN, GEMM16, REPACK16, TRANSPOSE, ALL_GATHER, SPLIT_B, OPERATOR } kind = KERNEL;
   std::string label;                  // op names, for profiling and error text
   // KERNEL
   int kernel = -1;                    // index into Executable::kernels
@@ -82,6 +83,8 @@ struct Step {
   // REPACK16: args = {dst, src}; iparams = {rows, cols, dst_ld, src_ld}
   // TRANSPOSE: args = {dst, src}; iparams = {element bytes, batch, rows, cols, dst_ld, dst batch stride, dst offset (elements)}
   Gemm16Launch g16;
+  // OPERATOR: args = {results, operands, [scratch]}; n_outs results, the scratch is the last when op.scratch_bytes > 0
+  OperatorLaunch op;
   // MEMCPY: args = {dst, src}; MEMSET: args = {dst}
   size_t bytes = 0;
   // WHILE: sub[0] = cond, sub[1] = body; state/init/next slot lists; pred slot

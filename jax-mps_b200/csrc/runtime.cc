@@ -730,7 +730,7 @@ b200_error* run_plan(ExecCtx& x, const Plan& plan);
 // Whether a kernel of the plan has a bounded wait (tensor-core pipelines; data-dependent loops, which are bounded in time).
 bool waits_inside(const Plan& plan) {
   for (const Step& s : plan.steps) {
-    if ((s.kind == Step::IGEMM && !s.ig.fma.split) || s.kind == Step::GEMM16 || (s.kind == Step::WHILE && s.trip_count < 0)) return true;
+    if ((s.kind == Step::IGEMM && !s.ig.fma.split) || s.kind == Step::GEMM16 || (s.kind == Step::OPERATOR && s.op.waits) || (s.kind == Step::WHILE && s.trip_count < 0)) return true;
     for (auto& p : s.sub)
       if (p && waits_inside(*p)) return true;
   }
@@ -927,6 +927,12 @@ class Recorder {
         return true;
       case Step::SCATTER:
         for (size_t k = 0; k < s.args.size(); k++) add(k < 3 ? reads_ : writes_, s.args[k]);
+        return true;
+      case Step::OPERATOR:
+        for (size_t k = 0; k < s.args.size(); k++) {
+          if ((int)k < s.n_outs || (s.op.scratch_bytes > 0 && k + 1 == s.args.size())) add(writes_, s.args[k]);
+          else if (!is_const(s.args[k])) add(reads_, s.args[k]);
+        }
         return true;
       default: return false;
     }
@@ -1233,6 +1239,16 @@ b200_error* run_step(ExecCtx& x, const Step& s) {
         return make_error(B200_INTERNAL, "launch of " + s.label + " failed: " + (why ? why : cudaGetErrorString(e)));
       return nullptr;
     }
+    case Step::OPERATOR: {
+      void* at[16];
+      size_t n = s.args.size();
+      if (n > 16) return make_error(B200_INTERNAL, "operator with more than 16 arguments");
+      for (size_t k = 0; k < n; k++) at[k] = x.ptrs[s.args[k]];
+      const char* why = nullptr;
+      cudaError_t e = launch_operator(s.op, at, s.op.scratch_bytes > 0 ? at[n - 1] : nullptr, c->error_flag, st, &x.launches, &why);
+      if (e != cudaSuccess) return make_error(B200_INTERNAL, "launch of " + s.label + " failed: " + (why ? why : cudaGetErrorString(e)));
+      return nullptr;
+    }
     case Step::TRANSPOSE: {
       char* dst = (char*)x.ptrs[s.args[0]] + s.iparams[6] * s.iparams[0];
       cudaError_t e = launch_transpose2d(dst, x.ptrs[s.args[1]], (int)s.iparams[0], s.iparams[1], s.iparams[2], s.iparams[3],
@@ -1414,6 +1430,7 @@ b200_error* run_step(ExecCtx& x, const Step& s) {
         set_programmatic_launch(false);
         set_igemm_programmatic_launch(false);
         set_gemm32_programmatic_launch(false);
+        set_operators_programmatic_launch(false);
         set_tile32_programmatic_launch(false);
         cudaError_t ce = cudaStreamBeginCapture(st, cudaStreamCaptureModeRelaxed);
         if (ce != cudaSuccess) fail(ce, "begin capture");
@@ -1469,6 +1486,7 @@ b200_error* run_step(ExecCtx& x, const Step& s) {
         set_programmatic_launch(!c->sw.no_pdl);
         set_igemm_programmatic_launch(!c->sw.no_pdl && !getenv("B200_NO_IGEMM_PDL"));
         set_gemm32_programmatic_launch(!c->sw.no_pdl);
+        set_operators_programmatic_launch(!c->sw.no_pdl);
         set_tile32_programmatic_launch(!c->sw.no_pdl);
         if (graph) cudaGraphDestroy(graph);
         const int recorded = x.launches - before;
@@ -1849,6 +1867,7 @@ b200_error* create_client(const b200_client_options* o, ncclComm_t given_comm, b
   set_programmatic_launch(!c->sw.no_pdl);
   set_igemm_programmatic_launch(!c->sw.no_pdl && !getenv("B200_NO_IGEMM_PDL"));
   set_gemm32_programmatic_launch(!c->sw.no_pdl);
+  set_operators_programmatic_launch(!c->sw.no_pdl);
         set_tile32_programmatic_launch(!c->sw.no_pdl);
   if (!driver().ok) return make_error(B200_FAILED_PRECONDITION, driver().error);
   if (c->nprocs > 1) {
@@ -3011,6 +3030,134 @@ b200_error* b200_matmul_f32_static_scratch(const float* a, const float* b, float
     return make_error(B200_INVALID_ARGUMENT, msg + " (m=" + std::to_string(m) + ", n=" + std::to_string(n) + ", limit " +
                                                  std::to_string(b200::static_scratch_bytes()) + " bytes)");
   return make_error(B200_INTERNAL, "static-scratch product failed: " + msg);
+}
+
+// ---- moves inside a paged cache --------------------------------------------------------------
+namespace {
+
+// Checks of a cache that both calls make; `shape` gets what the kernels need.
+b200_error* cache_shape(b200_client* c, const b200_buffer* cache, CacheShape* shape) {
+  if (!c || !cache) return make_error(B200_INVALID_ARGUMENT, "null argument");
+  if (cache->client != c) return make_error(B200_INVALID_ARGUMENT, "the cache lives on another client");
+  if (cache->deleted) return make_error(B200_INVALID_ARGUMENT, "the cache has been deleted or donated");
+  if (cache->dtype != B200_F32 && cache->dtype != B200_BF16 && cache->dtype != B200_F16)
+    return make_error(B200_INVALID_ARGUMENT, "a cache has to be f32, bf16 or f16");
+  const auto& d = cache->dims;
+  if (d.size() != 6 || d[1] != 2)
+    return make_error(B200_INVALID_ARGUMENT, "a cache has to be [layers, 2, pages, page size, key-value heads, features]");
+  shape->planes = d[0] * 2;
+  shape->pages = d[2];
+  shape->page = d[3];
+  shape->token = d[4] * d[5] * (cache->dtype == B200_F32 ? 4 : 2);
+  if (shape->token % 16) return make_error(B200_INVALID_ARGUMENT, "a token's keys of one layer have to be a multiple of 16 bytes");
+  if (shape->planes > 65535) return make_error(B200_INVALID_ARGUMENT, "a cache of more than 32767 layers");
+  if (shape->pages > INT32_MAX || shape->page > INT32_MAX || shape->pages * shape->page > INT32_MAX)
+    return make_error(B200_INVALID_ARGUMENT, "a cache of 2^31 positions and more");
+  return nullptr;
+}
+
+// Whether a non-negative index comes twice.
+bool repeats(const int32_t* index, size_t n, size_t stride) {
+  std::vector<int32_t> v;
+  v.reserve(n);
+  for (size_t k = 0; k < n; k++)
+    if (index[k * stride] >= 0) v.push_back(index[k * stride]);
+  std::sort(v.begin(), v.end());
+  return std::adjacent_find(v.begin(), v.end()) != v.end();
+}
+
+// In front of a change of `b` on the compute stream, and behind it.
+b200_error* before_change(b200_client* c, b200_buffer* b) {
+  CUDA_TRY(wait_for_copy(c, b));
+  for (auto& r : b->reads) CUDA_TRY(cudaStreamWaitEvent(c->compute, r->ev, 0));
+  b->reads.clear();
+  return nullptr;
+}
+b200_error* after_change(b200_client* c, b200_buffer* b, int launches) {
+  c->launches += launches;
+  CUDA_TRY(record_ready(c, c->compute, &b->ready));
+  b->ready_on = c->compute;
+  c->tail = b->ready.get();
+  return nullptr;
+}
+
+}  // namespace
+
+b200_error* b200_cache_write_pages(b200_client* c, b200_buffer* cache, b200_buffer* rows, const int32_t* slots, size_t n) try {
+  CacheShape shape;
+  if (auto* e = cache_shape(c, cache, &shape)) return e;
+  if (!rows || (n && !slots)) return make_error(B200_INVALID_ARGUMENT, "null argument");
+  if (rows->client != c) return make_error(B200_INVALID_ARGUMENT, "the rows live on another client");
+  if (rows->deleted) return make_error(B200_INVALID_ARGUMENT, "the rows have been deleted or donated");
+  const auto& d = cache->dims;
+  if (rows->dtype != cache->dtype || rows->dims != std::vector<int64_t>{d[0], 2, (int64_t)n, d[4], d[5]})
+    return make_error(B200_INVALID_ARGUMENT, "rows have to be [layers, 2, slots, key-value heads, features] of the cache's type and sizes");
+  for (size_t k = 0; k < n; k++)
+    if (slots[k] >= shape.pages * shape.page)
+      return make_error(B200_INVALID_ARGUMENT, "slot " + std::to_string(slots[k]) + " of row " + std::to_string(k) + " lies behind the cache, which has " +
+                                                   std::to_string(shape.pages * shape.page));
+  if (repeats(slots, n, 1)) return make_error(B200_INVALID_ARGUMENT, "two rows for one slot");
+  if (!n || !rows->bytes) return nullptr;
+  std::lock_guard<std::recursive_mutex> lock(c->mu);
+  if (auto* e = set_device(c)) return e;
+  if (auto* e = before_change(c, cache)) return e;
+  CUDA_TRY(wait_for_copy(c, rows));
+  int launches = 0;
+  CUDA_TRY(launch_write_pages(shape, cache->ptr, rows->ptr, slots, (long long)n, c->compute, &launches));
+  // an execution that gave up on a wait left its mark on the rows: what was made of them carries it too
+  if (rows->status && !(cache->status && cache->status->failed())) cache->status = rows->status;
+  return after_change(c, cache, launches);
+} catch (const std::exception& e) {
+  return make_error(B200_INTERNAL, std::string("write_pages: ") + e.what());
+}
+
+b200_error* b200_cache_copy_pages(b200_client* c, b200_buffer* cache, const int32_t* pairs, size_t n) try {
+  CacheShape shape;
+  if (auto* e = cache_shape(c, cache, &shape)) return e;
+  if (n && !pairs) return make_error(B200_INVALID_ARGUMENT, "null argument");
+  for (size_t k = 0; k < 2 * n; k++)
+    if (pairs[k] < 0 || pairs[k] >= shape.pages)
+      return make_error(B200_INVALID_ARGUMENT, "page " + std::to_string(pairs[k]) + " of pair " + std::to_string(k / 2) + " is not in the cache, which has " +
+                                                   std::to_string(shape.pages));
+  if (repeats(pairs + 1, n, 2)) return make_error(B200_INVALID_ARGUMENT, "two pairs for one destination");
+  if (!n || !cache->bytes) return nullptr;
+  // A source that another pair overwrites is set aside first: the pairs of a launch run in no order. Everything else is copied once.
+  std::vector<int> moves, staged, sources;
+  std::vector<int32_t> written;
+  for (size_t k = 0; k < n; k++)
+    if (pairs[2 * k] != pairs[2 * k + 1]) written.push_back(pairs[2 * k + 1]);
+  std::sort(written.begin(), written.end());
+  for (size_t k = 0; k < n; k++) {
+    const int src = pairs[2 * k], dst = pairs[2 * k + 1];
+    if (src == dst) continue;
+    moves.push_back(src);
+    moves.push_back(dst);
+    const bool aside = std::binary_search(written.begin(), written.end(), src);
+    staged.push_back(aside ? (int)sources.size() : -1);
+    if (aside) sources.push_back(src);
+  }
+  if (moves.empty()) return nullptr;
+  std::lock_guard<std::recursive_mutex> lock(c->mu);
+  if (auto* e = set_device(c)) return e;
+  void* stage = nullptr;
+  const size_t stage_bytes = sources.size() * (size_t)(shape.planes * shape.page * shape.token);
+  if (stage_bytes)
+    if (auto* e = device_alloc(c, stage_bytes, c->compute, &stage)) return e;
+  int launches = 0;
+  auto work = [&]() -> b200_error* {
+    if (auto* e = before_change(c, cache)) return e;
+    if (stage) CUDA_TRY(launch_stage_pages(shape, cache->ptr, stage, sources.data(), (long long)sources.size(), c->compute, &launches));
+    CUDA_TRY(launch_copy_pages(shape, cache->ptr, moves.data(), staged.data(), stage, (long long)staged.size(), c->compute, &launches));
+    return after_change(c, cache, launches);
+  };
+  b200_error* err = work();
+  if (stage) {                                   // freed in the order of the compute stream
+    block_free(c, stage, stage_bytes);
+    c->note_free(std::max<size_t>(stage_bytes, 16));
+  }
+  return err;
+} catch (const std::exception& e) {
+  return make_error(B200_INTERNAL, std::string("copy_pages: ") + e.what());
 }
 
 }  // extern "C"

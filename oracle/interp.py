@@ -24,10 +24,12 @@ every op. Floating-point reductions accumulate in float64.
 from __future__ import annotations
 
 import math
+import re
 
 import numpy as np
 
 from . import mlir_text as mt
+from . import operators
 from .mlir_text import Block, Module, Op, TType, attr_i64s, attr_int, enum_word, struct_fields
 
 FLOATS = ("f32", "bf16", "f16", "f64")
@@ -961,6 +963,10 @@ class Interp:
                     return [_UNARY[fn](x[0].astype(np.float64))]
             if hasattr(self, "op_" + fn):
                 return getattr(self, "op_" + fn)(op, x, env)
+        if tgt.startswith("b200."):
+            text = op.attrs.get("backend_config", op.attrs.get("mhlo.backend_config", ""))
+            config = {k: float(v) if k == "scale" else int(v) for k, v in re.findall(r"(\w+) = ([-+.\w]+) : \w+", text)}
+            return operators.run(tgt, x, config)
         raise NotImplementedError(f"oracle: custom_call {tgt}")
 
     # ---- collectives ---------------------------------------------------------------------------------

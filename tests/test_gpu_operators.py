@@ -1,0 +1,481 @@
+"""Operators that programs name as custom calls, and the moves inside a paged cache, against their definitions in 64 bits.
+
+Tolerances count roundings. u is half a step of the type, e = 2^-24. A result is rounded once (u |out|). A score is a sum of D products
+(at most (D + 4) e of the sum of its absolute terms, `top`), goes through exp2 with an argument whose own rounding is at most
+4 e top and whose function is good to 2^-22: a weight is off by d = (D + 8) e top + 2^-22 relative, the normaliser by as much, and
+a sum over n positions by n e: 2 d + 2 n e of sum_j w_j |v_j| (`mag`). The tensor-core kernels of 16-bit data round the weights to 16
+bits for the second product: u mag more, or u^2 mag where they go in two pieces."""
+import numpy as np
+import pytest
+
+from b200.pages import PagedCache
+from b200.shlo.builder import Builder
+from oracle import interp, operators
+
+pytestmark = pytest.mark.gpu
+
+U = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}
+E = 2.0 ** -24
+
+
+def rounded(a, dt):
+    a = np.asarray(a, np.float32)
+    return a if dt == "f32" else a.astype(np.float16).astype(np.float32) if dt == "f16" else interp.round_bf16(a)
+
+
+def put(client, a, dt):
+    a = np.asarray(a)
+    if dt in U:
+        a = a.astype(np.float16 if dt == "f16" else np.float32)
+    return client.buffer_from_host(a, dtype="bf16" if dt == "bf16" else None)
+
+
+def run(client, build, arrays, dts):
+    """Arguments of `build(builder, *vals)` from arrays; the results as NumPy arrays, from two calls that have to agree bit for bit."""
+    b = Builder()
+    outs = build(b, *[b.arg(np.shape(a), dt) for a, dt in zip(arrays, dts)])
+    exe = client.compile(b.module(outs if isinstance(outs, list) else [outs]))
+    bufs = [put(client, a, dt) for a, dt in zip(arrays, dts)]
+    first, second = ([np.asarray(o.to_numpy()) for o in exe.execute(bufs)] for _ in range(2))
+    for x, y in zip(first, second):
+        np.testing.assert_array_equal(x, y)
+    return first
+
+
+def attention_tolerance(want, mag, top, n, D, dt, weights):
+    u = U[dt]
+    d = (D + 8) * E * top + 2.0 ** -22
+    return u * np.abs(want) + mag * (2 * d + 2 * n * E + weights) + (2.0 ** -25 if dt == "f16" else 0.0)
+
+
+def paged_case(rng, lens, H, KH, D, S, dt, new, layers=1, spare=2):
+    B = len(lens)
+    width = max(1, max(-(-n // S) for n in lens))
+    pages = sum(-(-n // S) for n in lens) + spare
+    order, table, at = rng.permutation(pages), np.full((B, width), -1, np.int32), 0
+    for b, n in enumerate(lens):
+        m = -(-n // S)
+        table[b, :m] = order[at:at + m]
+        at += m
+    q = rounded(rng.standard_normal((B, H, D)), dt)
+    cache = rounded(rng.standard_normal((layers, 2, pages, S, KH, D)), dt)
+    fresh = rounded(rng.standard_normal((2, B, KH, D)), dt) if new else None
+    return q, cache, table, np.asarray(lens, np.int32), fresh
+
+
+def check_paged(client, q, cache, table, lengths, fresh, dt, **kw):
+    arrays, dts = [q, cache, table, lengths], [dt, dt, "i32", "i32"]
+    if fresh is not None:
+        arrays.append(fresh)
+        dts.append(dt)
+    got = run(client, lambda b, q, c, t, n, new=None: b.paged_attention(q, c, t, n, new=new, **kw), arrays, dts)[0]
+    want, mag, top = operators.paged_attention(q, cache, table, lengths, fresh, bounds=True, **kw)
+    tol = attention_tolerance(want, mag, top, int(max(lengths.max(initial=0), 0)) + 1, q.shape[-1], dt, 0.0 if dt == "f32" else U[dt])
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (float(np.abs(got - want)[bad].max()), np.argwhere(bad)[:5].tolist(), int(bad.sum()))
+    return got
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("H,KH,D,S", [(8, 1, 256, 16), (4, 4, 64, 5), (6, 2, 128, 64), (7, 1, 72, 1), (32, 2, 96, 24), (3, 3, 8, 7), (24, 1, 192, 32), (2, 1, 248, 3)])
+@pytest.mark.parametrize("new", [False, True])
+def test_paged_attention_heads_and_pages(client, dt, H, KH, D, S, new):
+    rng = np.random.default_rng(H * D + S + new)
+    check_paged(client, *paged_case(rng, [0, 1, 2, 15, 16, 17, 100, 33], H, KH, D, S, dt, new), dt)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 3), (2, 1), (16, 4), (100, 0), (130, 20), (1000, 5)])
+@pytest.mark.parametrize("new", [False, True])
+def test_paged_attention_window_and_sinks(client, dt, window, sinks, new):
+    rng = np.random.default_rng(window)
+    check_paged(client, *paged_case(rng, [0, 1, 3, 16, 99, 131, 260, 700], 4, 2, 64, 8, dt, new), dt, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lens", [[127], [128], [129], [1023, 1], [3001, 0, 64, 2000], [40, 5000] + [17] * 37])
+def test_paged_attention_split_over_the_length(client, dt, lens):
+    rng = np.random.default_rng(sum(lens))
+    check_paged(client, *paged_case(rng, lens, 4, 1, 64, 16, dt, True), dt)
+
+
+def test_paged_attention_many_sequences(client):
+    rng = np.random.default_rng(5)
+    check_paged(client, *paged_case(rng, rng.integers(0, 40, 1500).tolist(), 2, 1, 8, 4, "bf16", True), "bf16")
+
+
+def test_paged_attention_layer_scale_and_shared_pages(client):
+    rng = np.random.default_rng(11)
+    q, cache, table, lengths, fresh = paged_case(rng, [30, 45, 45], 4, 2, 64, 16, "bf16", True, layers=3)
+    table[2, :2] = table[1, :2]                                    # a fork: two sequences read the same pages
+    for layer in range(3):
+        check_paged(client, q, cache, table, lengths, fresh, "bf16", layer=layer, scale=0.3)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_paged_attention_reads_nothing_that_is_hidden(client, dt):
+    """NaN and infinities in slots behind a sequence, in pages of others, behind the window; lengths and pages out of range."""
+    rng = np.random.default_rng(2)
+    S, lens = 8, [21, 5, 0, 40]
+    q, cache, table, lengths, fresh = paged_case(rng, lens, 4, 2, 64, S, dt, True)
+    seen = np.zeros(cache.shape[2:4], bool)
+    for b, n in enumerate(lens):
+        for j in operators.visible(n, n, 12, 2):
+            seen[table[b, j // S], j % S] = True
+    cache[:, 0][:, ~seen] = np.nan
+    cache[:, 1][:, ~seen] = np.inf
+    check_paged(client, q, cache, table, lengths, fresh, dt, window=12, sinks=2)
+    # lengths below zero and above the table's room
+    check_paged(client, q, np.nan_to_num(cache, posinf=1.0), np.abs(table), np.array([-3, 1000, 2**31 - 1, -2**31], np.int32), fresh, dt)
+
+
+@pytest.mark.parametrize("new", [False, True])
+def test_paged_attention_leaves_out_pages_that_are_not_there(client, new):
+    rng = np.random.default_rng(4)
+    q, cache, table, lengths, fresh = paged_case(rng, [40, 40, 40], 4, 2, 64, 8, "bf16", new)
+    table[0, 1], table[1, 3], table[2, :] = -7, cache.shape[2], 2**31 - 1
+    check_paged(client, q, cache, table, lengths, fresh, "bf16")
+
+
+def test_paged_attention_scores_at_the_edge(client):
+    """Large scores, one position that takes all of the weight, infinities in a visible key (as the definition gives them)."""
+    rng = np.random.default_rng(8)
+    q, cache, table, lengths, fresh = paged_case(rng, [50, 50], 2, 1, 64, 16, "f32", False)
+    check_paged(client, q * 30, cache, table, lengths, fresh, "f32")
+    cache[0, 0, table[0, 0], 3, 0, :] = np.where(q[0, 0] > 0, -3e38, 3e38)          # a score of minus infinity: no weight
+    got = run(client, lambda b, q, c, t, n: b.paged_attention(q, c, t, n), [q[:1, :1], cache, table[:1], lengths[:1]], ["f32", "f32", "i32", "i32"])[0]
+    with np.errstate(all="ignore"):
+        want = operators.paged_attention(q[:1, :1], cache, table[:1], lengths[:1])
+    np.testing.assert_allclose(got, want, rtol=1e-4, atol=1e-5)
+    cache[0, 0, table[0, 0], 3, 0, :] = np.nan
+    got = run(client, lambda b, q, c, t, n: b.paged_attention(q, c, t, n), [q, cache, table, lengths], ["f32", "f32", "i32", "i32"])[0]
+    assert np.isnan(got[0]).all() and np.isfinite(got[1]).all()
+
+
+def test_paged_attention_of_nothing(client):
+    for B, W in ((0, 3), (2, 0)):
+        q, cache = np.ones((B, 2, 8), np.float32), np.ones((1, 2, 0 if W == 0 else 4, 2, 1, 8), np.float32)
+        args = [q, cache, np.zeros((B, W), np.int32), np.full(B, 4, np.int32)]
+        got = run(client, lambda b, *a: b.paged_attention(*a), args, ["f32", "f32", "i32", "i32"])[0]
+        assert got.shape == q.shape and (got == 0).all()
+
+
+# ---- prompts ------------------------------------------------------------------------------------------
+def check_prompt(client, q, k, v, lengths, dt, **kw):
+    arrays, dts = [q, k, v] + ([lengths] if lengths is not None else []), [dt] * 3 + ["i32"]
+    got = run(client, lambda b, q, k, v, n=None: b.window_attention(q, k, v, n, **kw), arrays, dts)[0]
+    known = [np.where(np.isfinite(t), t, 0.0) for t in (q, k, v)]
+    want, mag, top = operators.window_attention(*known, lengths, bounds=True, **kw)
+    tol = attention_tolerance(want, mag, top, q.shape[1], q.shape[-1], dt, 0.0 if dt == "f32" else U[dt])
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (float(np.nanmax(np.abs(got - want)[bad])), np.argwhere(bad)[:5].tolist(), int(bad.sum()))
+
+
+def prompt_case(rng, B, T, H, KH, D, dt):
+    return [rounded(rng.standard_normal(s), dt) for s in ((B, T, H, D), (B, T, KH, D), (B, T, KH, D))]
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("H,KH,D", [(2, 1, 256), (3, 3, 64), (4, 2, 128), (2, 1, 72), (1, 1, 192), (2, 2, 8), (2, 1, 248)])
+@pytest.mark.parametrize("T", [1, 77, 130])
+def test_window_attention_heads_and_lengths(client, dt, H, KH, D, T):
+    rng = np.random.default_rng(H * D + T)
+    check_prompt(client, *prompt_case(rng, 1, T, H, KH, D, dt), None, dt)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 2), (5, 0), (64, 1), (100, 4), (129, 130), (300, 16), (1000, 0)])
+def test_window_attention_windows(client, dt, window, sinks):
+    rng = np.random.default_rng(window + sinks)
+    check_prompt(client, *prompt_case(rng, 1, 413, 2, 1, 64, dt), None, dt, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_window_attention_long_rows_of_tiles(client, dt, D):
+    rng = np.random.default_rng(D)
+    check_prompt(client, *prompt_case(rng, 1, 1100, 1, 1, D, dt), None, dt)
+    check_prompt(client, *prompt_case(rng, 1, 1100, 1, 1, D, dt), None, dt, window=200, sinks=3)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_window_attention_padded_batch(client, dt):
+    rng = np.random.default_rng(9)
+    lengths = np.array([150, 0, 1, 64, 129, -4, 2000], np.int32)
+    q, k, v = prompt_case(rng, 7, 150, 2, 1, 64, dt)
+    for b, n in enumerate(lengths):
+        n = min(max(n, 0), 150)
+        q[b, n:], k[b, n:], v[b, n:] = np.nan, np.inf, np.nan          # nobody reads what stands behind a sequence
+    check_prompt(client, q, k, v, lengths, dt, window=70, sinks=2, scale=0.2)
+
+
+# ---- log probabilities ---------------------------------------------------------------------------------
+def check_probs(client, x, tokens, top, dt, cotangents=None):
+    R, V = x.shape
+    arrays, dts = [x, np.asarray(tokens, np.int32)], [dt, "i32"]
+    if cotangents is not None:
+        arrays += cotangents
+        dts += ["f32"] * 3
+
+    def build(b, x, t, *g):
+        outs = b.token_log_probs(x, t, top=top)
+        if g:
+            total = b.add(b.add(b.mul(outs[0], g[0]), b.mul(outs[1], g[1])), b.mul(outs[2], g[2]))
+            outs = outs + b.grad(b.reduce_sum(total, (0,)), [x])
+        return outs
+    got = run(client, build, arrays, dts)
+    want = operators.token_log_probs(x, tokens, top)
+    # m + log s: exponentials good to 2^-21 (argument rounding and function), sums of V terms in pairs and threads' runs (V / 256 + 16 e),
+    # and the result's own rounding; the entropy's terms p (x - m) carry the same relative errors times the span of the logits that count
+    finite = np.where(np.isfinite(x), x, 0.0)
+    span = float(np.abs(finite).max()) * 2 + 1
+    rel = 2.0 ** -21 + (V / 256 + 16) * E
+    for g, w, scale in zip(got[:3], want[:3], (1.0, span, 1.0)):
+        tol = scale * rel * 2 + 4 * E * (np.abs(finite).max() + np.abs(np.where(np.isfinite(w), w, 0.0)))
+        same = (g == w) | (np.isnan(g) & np.isnan(w))
+        with np.errstate(invalid="ignore"):
+            assert (same | (np.abs(g - w) <= tol)).all(), (g, w, tol)
+    if top:
+        np.testing.assert_array_equal(got[4], want[4])
+        with np.errstate(invalid="ignore"):
+            close = np.abs(got[3] - want[3]) <= 2 * rel + 8 * E * (np.abs(finite).max() + 20)
+        assert (close | (got[3] == want[3]) | (np.isnan(got[3]) & np.isnan(want[3]))).all()
+    if cotangents is not None:
+        dx, ref = got[-1], operators.token_log_probs_grad(x, tokens, *cotangents)
+        gl, gh, gn = (np.abs(c)[:, None] for c in cotangents)
+        p = np.exp(np.asarray(x, np.float64) - want[2][:, None])
+        off = rel * 3 + 8 * E * (np.abs(finite).max() + 20)                 # of a probability: that of its exponent
+        size = p * (gl + gn + gh * (span + 20))
+        assert (np.abs(dx - ref) <= U[dt] * np.abs(ref) + size * off * 2 + 4 * E * (np.abs(ref) + size) + (2.0 ** -25 if dt == "f16" else 1e-40)).all()
+    return got
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("R,V", [(1, 1), (3, 7), (5, 255), (2, 1000), (9, 1031), (4, 30522), (1, 256000), (300, 512)])
+def test_token_log_probs(client, dt, R, V):
+    rng = np.random.default_rng(V + R)
+    x = rounded(rng.standard_normal((R, V)) * 4, dt)
+    tokens = rng.integers(0, V, R)
+    tokens[::3] = -1
+    tokens[1::5] = V
+    check_probs(client, x, tokens, min(V, 5), dt)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("top", [1, 2, 31, 64, 128])
+@pytest.mark.parametrize("V", [128, 5003, 66000])
+def test_alternatives_with_equal_logits(client, dt, top, V):
+    """Few distinct values: equal ones by their number; rows in order and against it; a row of one value."""
+    rng = np.random.default_rng(top)
+    rows = [rng.integers(0, 3, V), np.arange(V) // 7, -np.arange(V) // 5, np.zeros(V), rng.integers(0, 50, V) - 0.0, np.where(np.arange(V) % 97, -0.0, 0.0)]
+    check_probs(client, rounded(np.stack(rows) / 4.0, dt), np.arange(6), top, dt)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_token_log_probs_of_masked_vocabularies(client, dt):
+    """Minus infinity, the type's lowest value, plus infinity, NaN, rows that leave one token or none."""
+    rng = np.random.default_rng(1)
+    V, low = 3001, {"f32": -3.4028235e38, "bf16": -3.3895314e38, "f16": -65504.0}[dt]
+    x = rounded(rng.standard_normal((9, V)), dt)
+    x[0, rng.random(V) < 0.9] = -np.inf
+    x[1, rng.random(V) < 0.9] = low
+    x[2] = -np.inf
+    x[2, 1234] = 2.0
+    x[3] = low
+    x[4] = -np.inf
+    x[5, 17] = np.inf
+    x[6, 2900] = np.nan
+    x[7, :10] = np.nan
+    x[8, 1:] = low
+    tokens = np.array([int(np.argmax(x[0])), 3, 1234, 5, 7, 17, 3, 2, 0])
+    with np.errstate(invalid="ignore"):
+        got = check_probs_special(client, x, tokens, 20, dt)
+    assert got[0][2] == 0.0 and got[1][2] == 0.0
+    assert np.isnan(got[0][[4, 5, 6, 7]]).all()
+
+
+def check_probs_special(client, x, tokens, top, dt):
+    got = run(client, lambda b, x, t: b.token_log_probs(x, t, top=top), [x, np.asarray(tokens, np.int32)], [dt, "i32"])
+    want = operators.token_log_probs(x, tokens, top)
+    np.testing.assert_array_equal(got[4], want[4])
+    for g, w in zip(got[:4], want[:4]):
+        np.testing.assert_array_equal(np.isnan(g), np.isnan(w))
+        ok = ~np.isnan(w)
+        np.testing.assert_allclose(g[ok], w[ok], rtol=1e-5, atol=2e-5)
+    return got
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("R,V", [(1, 1), (7, 65), (5, 1000), (3, 30522), (2, 70001), (64, 2048)])
+def test_gradient_of_token_log_probs(client, dt, R, V):
+    rng = np.random.default_rng(V)
+    x = rounded(rng.standard_normal((R, V)) * 3, dt)
+    tokens = rng.integers(0, V, R)
+    tokens[::4] = -100
+    g = [rng.standard_normal(R).astype(np.float32) for _ in range(3)]
+    check_probs(client, x, tokens, 0, dt, g)
+
+
+def test_gradient_where_the_vocabulary_is_masked(client):
+    rng = np.random.default_rng(6)
+    x = (rng.standard_normal((4, 999)) * 2).astype(np.float32)
+    x[:, ::2] = -np.inf
+    tokens = np.array([1, 3, 5, -1])
+    g = [rng.standard_normal(4).astype(np.float32) for _ in range(3)]
+    got = check_probs(client, x, tokens, 0, "f32", g)
+    assert (got[-1][:, ::2] == 0).all()
+
+
+def test_log_probs_of_no_rows(client):
+    got = run(client, lambda b, x, t: b.token_log_probs(x, t, top=2), [np.zeros((0, 10), np.float32), np.zeros(0, np.int32)], ["f32", "i32"])
+    assert [g.shape for g in got] == [(0,)] * 3 + [(0, 2)] * 2
+
+
+# ---- moves inside a cache ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("L,P,S,KH,D,n", [(1, 3, 4, 1, 8, 1), (2, 10, 16, 2, 64, 50), (18, 6, 16, 1, 256, 3), (3, 200, 24, 3, 72, 4000), (1, 5000, 1, 1, 8, 2500)])
+def test_write_pages(client, dt, L, P, S, KH, D, n):
+    rng = np.random.default_rng(n)
+    cache, rows = rounded(rng.standard_normal((L, 2, P, S, KH, D)), dt), rounded(rng.standard_normal((L, 2, n, KH, D)), dt)
+    slots = rng.permutation(P * S)[:n].astype(np.int32)
+    slots[rng.random(n) < 0.2] = -1
+    buf, src = put(client, cache, dt), put(client, rows, dt)
+    client.write_pages(buf, src, slots)
+    np.testing.assert_array_equal(buf.to_numpy(), operators.write_pages(cache, rows, slots))
+    np.testing.assert_array_equal(src.to_numpy(), rows)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("L,P,S,KH,D,n", [(1, 4, 2, 1, 8, 2), (5, 60, 16, 2, 64, 30), (2, 3000, 3, 1, 24, 1400), (1, 40, 64, 4, 128, 20)])
+def test_copy_pages(client, dt, L, P, S, KH, D, n):
+    rng = np.random.default_rng(n)
+    cache = rounded(rng.standard_normal((L, 2, P, S, KH, D)), dt)
+    # any sources, distinct destinations: chains, exchanges, pages onto themselves, one source for many
+    pairs = np.stack([rng.integers(0, P, n), rng.permutation(P)[:n]], 1).astype(np.int32)
+    buf = put(client, cache, dt)
+    client.copy_pages(buf, pairs)
+    np.testing.assert_array_equal(buf.to_numpy(), operators.copy_pages(cache, pairs))
+
+
+@pytest.mark.parametrize("pairs", [[(0, 1), (1, 0)], [(i + 1, i) for i in range(999)], [(i, i + 1) for i in range(999)], [(i, (i + 1) % 1000) for i in range(1000)], [(5, 5)], []])
+def test_copy_pages_chains(client, pairs):
+    cache = np.arange(1000 * 16, dtype=np.float32).reshape(1, 2, 1000, 1, 1, 8)
+    buf = put(client, cache, "f32")
+    client.copy_pages(buf, pairs)
+    np.testing.assert_array_equal(buf.to_numpy(), operators.copy_pages(cache, pairs))
+
+
+def test_moves_refuse(client):
+    import b200
+    cache = put(client, np.zeros((2, 2, 4, 2, 1, 8)), "bf16")
+    rows = put(client, np.zeros((2, 2, 3, 1, 8)), "bf16")
+
+    def refuse(why, call):
+        with pytest.raises(b200.B200Error) as e:
+            call()
+        assert e.value.code == b200.INVALID_ARGUMENT and why in str(e.value), str(e.value)
+    refuse("two rows for one slot", lambda: client.write_pages(cache, rows, [1, 2, 1]))
+    refuse("behind the cache", lambda: client.write_pages(cache, rows, [1, 2, 8]))
+    refuse("rows have to be", lambda: client.write_pages(cache, rows, [1, 2]))
+    refuse("rows have to be", lambda: client.write_pages(cache, put(client, np.zeros((2, 2, 3, 1, 8)), "f16"), [1, 2, 3]))
+    refuse("rows have to be", lambda: client.write_pages(cache, cache, [1, 2, 3, 4]))
+    refuse("two pairs", lambda: client.copy_pages(cache, [(0, 1), (2, 1)]))
+    refuse("not in the cache", lambda: client.copy_pages(cache, [(0, 4)]))
+    refuse("not in the cache", lambda: client.copy_pages(cache, [(-1, 0)]))
+    refuse("a cache has to be", lambda: client.copy_pages(rows, [(0, 1)]))
+    refuse("f32, bf16 or f16", lambda: client.copy_pages(client.buffer_from_host(np.zeros((2, 2, 4, 2, 1, 8), np.int32)), [(0, 1)]))
+    refuse("multiple of 16 bytes", lambda: client.copy_pages(put(client, np.zeros((2, 2, 4, 2, 1, 4)), "bf16"), [(0, 1)]))
+    client.write_pages(cache, rows, [-1, -1, -1])
+    client.write_pages(cache, put(client, np.zeros((2, 2, 0, 1, 8)), "bf16"), [])
+    gone = put(client, np.zeros((2, 2, 4, 2, 1, 8)), "bf16")
+    gone.delete()
+    refuse("deleted", lambda: client.copy_pages(gone, [(0, 1)]))
+
+
+def test_moves_keep_their_place_among_executions_and_reads(client):
+    """A read that was started sees the cache as it was, an execution behind the change sees it as it is."""
+    rng = np.random.default_rng(0)
+    shape = (1, 2, 64, 16, 8, 128)
+    old = rng.standard_normal(shape).astype(np.float32)
+    b = Builder()
+    c = b.arg(shape, "f32")
+    twice = client.compile(b.module([b.mul(c, b.full(shape, 2.0, "f32"))]))
+    for _ in range(5):
+        buf, rows = put(client, old, "f32"), put(client, np.ones((1, 2, 16, 8, 128)), "f32")
+        before = twice.execute([buf])[0]
+        host = np.empty(shape, np.float32)
+        event = buf.to_host_async(host)
+        client.write_pages(buf, rows, np.arange(16))
+        client.copy_pages(buf, [(0, 63)])
+        behind = twice.execute([buf])[0]
+        event.wait()
+        new = operators.copy_pages(operators.write_pages(old, np.ones((1, 2, 16, 8, 128)), np.arange(16)), [(0, 63)])
+        np.testing.assert_array_equal(host, old)
+        np.testing.assert_array_equal(buf.to_numpy(), new)
+        np.testing.assert_array_equal(before.to_numpy(), 2 * old)
+        np.testing.assert_array_equal(behind.to_numpy(), 2 * new)
+
+
+def test_cache_of_more_than_32_bits(client):
+    """The last pages of a cache with 2^31 elements and more in each plane."""
+    KH, S, D, P = 8, 64, 256, 16400
+    assert P * S * KH * D > 2**31
+    cache = PagedCache(client, 1, P, S, KH, D)
+    rng = np.random.default_rng(0)
+    n = 70
+    rows = rounded(rng.standard_normal((1, 2, n, KH, D)), "bf16")
+    table = np.array([[P - 1, P - 2]], np.int32)
+    at = np.arange(n)
+    client.write_pages(cache.buffer, put(client, rows, "bf16"), table[0][at // S] * S + at % S)
+    client.copy_pages(cache.buffer, [(P - 1, 3), (P - 2, P - 5)])
+    q = rounded(rng.standard_normal((1, 16, D)), "bf16")
+    b = Builder()
+    a = [b.arg((1, 16, D), "bf16"), b.arg(cache.shape, "bf16"), b.arg((1, 2), "i32"), b.arg((1,), "i32")]
+    exe = client.compile(b.module([b.paged_attention(*a)]))
+    small = np.zeros((1, 2, 2, S, KH, D))
+    small[0].reshape(2, 2 * S, KH, D)[:, :n] = rows[0]
+    want, mag, top = operators.paged_attention(q, small, np.array([[0, 1]]), [n], bounds=True)
+    for t in (table, np.array([[3, P - 5]], np.int32)):
+        got = exe.execute([put(client, q, "bf16"), cache.buffer, client.buffer_from_host(t), client.buffer_from_host(np.array([n], np.int32))])[0].to_numpy()
+        assert (np.abs(got - want) <= attention_tolerance(want, mag, top, n, D, "bf16", U["bf16"])).all()
+    cache.buffer.delete()
+
+
+# ---- inside programs -----------------------------------------------------------------------------------------
+def test_operators_in_a_recorded_program_and_a_loop(client):
+    """Several operators whose scratch lives in one arena, replayed with other buffers, and one in a loop body."""
+    rng = np.random.default_rng(12)
+    q, cache, table, lengths, _ = paged_case(rng, [700, 20, 300], 4, 2, 64, 16, "f32", False)
+    b = Builder()
+    a = [b.arg(q.shape, "f32"), b.arg(cache.shape, "f32"), b.arg(table.shape, "i32"), b.arg(lengths.shape, "i32")]
+    outs, x = [], a[0]
+    for w in (0, 300, 150, 0):
+        x = b.paged_attention(x, *a[1:], window=w, sinks=2 if w else 0)
+        outs.append(b.mul(x, b.full(q.shape, 2.0, "f32")))
+    flat = b.reshape(x, (12, 64))
+    outs += b.token_log_probs(flat, b.reshape(b.concatenate([a[3]] * 4, 0), (12,)), top=3)
+    loop = b.while_([b.const(0, "i32"), a[0]], lambda s, i, v: s.compare(i, s.const(3, "i32"), "LT"),
+                    lambda s, i, v: [s.add(i, s.const(1, "i32")), s.paged_attention(v, a[1], a[2], a[3])])
+    text = b.module(outs + [loop[1]])
+    exe = client.compile(text)
+    for seed in range(3):
+        q2 = np.random.default_rng(seed).standard_normal(q.shape).astype(np.float32)
+        args = [q2, cache, table, lengths]
+        want = interp.run_text(text, args)
+        for _ in range(2):
+            got = [o.to_numpy() for o in exe.execute([client.buffer_from_host(v) for v in args])]
+            for g, w in zip(got, want):
+                np.testing.assert_allclose(g, w, rtol=1e-4, atol=1e-5)
+
+
+def test_two_calls_in_flight(client):
+    rng = np.random.default_rng(13)
+    cases = [paged_case(rng, [900, 33], 8, 2, 64, 16, "f32", False) for _ in range(2)]
+    b = Builder()
+    c = cases[0]
+    a = [b.arg(x.shape, dt) for x, dt in zip(c[:4], ("f32", "f32", "i32", "i32"))]
+    exe = client.compile(b.module([b.paged_attention(*a)]))
+    bufs = [[client.buffer_from_host(x) for x in c[:4]] for c in cases]
+    outs = [exe.execute(bufs[i % 2])[0] for i in range(10)]
+    for i, o in enumerate(outs):
+        np.testing.assert_allclose(o.to_numpy(), operators.paged_attention(*cases[i % 2][:4]), rtol=1e-4, atol=1e-5)

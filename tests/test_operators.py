@@ -1,0 +1,202 @@
+"""Operators that programs name as custom calls, and the bookkeeping of the paged cache: what needs no GPU."""
+import numpy as np
+import pytest
+
+import b200
+from b200.pages import PagedCache
+from b200.shlo.builder import Builder
+from oracle import interp, operators
+
+
+def paged_text(B=3, H=8, KH=2, D=64, L=2, P=5, S=16, W=4, dt="bf16", new=True, **kw):
+    b = Builder()
+    q, cache = b.arg((B, H, D), dt), b.arg((L, 2, P, S, KH, D), dt)
+    table, lengths = b.arg((B, W), "i32"), b.arg((B,), "i32")
+    n = b.arg((2, B, KH, D), dt) if new else None
+    return b.module([b.paged_attention(q, cache, table, lengths, new=n, **kw)])
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_programs_with_operators_compile(dt):
+    plan, _ = b200.compile_to_plan(paged_text(dt=dt, layer=1, window=20, sinks=4, scale=0.1))
+    assert "operator paged_attention" in plan
+    b = Builder()
+    q, k, v = b.arg((2, 33, 4, 64), dt), b.arg((2, 33, 2, 64), dt), b.arg((2, 33, 2, 64), dt)
+    plan, _ = b200.compile_to_plan(b.module([b.window_attention(q, k, v, window=7)]))
+    assert "operator window_attention" in plan
+    b = Builder()
+    x, t, g = b.arg((5, 1000), dt), b.arg((5,), "i32"), b.arg((5,), "f32")
+    lp, *rest = b.token_log_probs(x, t, top=3)
+    dx = b.grad(b.reduce_sum(b.mul(lp, g), (0,)), [x])[0]
+    assert (dx.shape, dx.dtype) == ((5, 1000), dt)
+    plan, _ = b200.compile_to_plan(b.module([lp, *rest, dx]))
+    assert "operator token_log_probs " in plan and "operator token_log_probs_grad" in plan
+
+
+def test_the_assembly_jax_prints():
+    # jax.ffi.ffi_call(...)(q, ...): the dictionary stands under one of two names
+    for attr in ("backend_config = {layer = 1 : i64, window = 5 : i64}, api_version = 4 : i32", "mhlo.backend_config = {layer = 1 : i64, window = 5 : i64}"):
+        text = f"""module @jit_f {{
+  func.func public @main(%arg0: tensor<1x2x8xf32>, %arg1: tensor<2x2x3x4x1x8xf32>, %arg2: tensor<1x2xi32>, %arg3: tensor<1xi32>) -> tensor<1x2x8xf32> {{
+    %0 = stablehlo.custom_call @b200.paged_attention(%arg0, %arg1, %arg2, %arg3) {{{attr}}} : (tensor<1x2x8xf32>, tensor<2x2x3x4x1x8xf32>, tensor<1x2xi32>, tensor<1xi32>) -> tensor<1x2x8xf32>
+    return %0 : tensor<1x2x8xf32>
+  }}
+}}"""
+        plan, _ = b200.compile_to_plan(text)
+        assert "operator paged_attention layer=1 window=5" in plan
+        rng = np.random.default_rng(0)
+        q, c = rng.standard_normal((1, 2, 8)).astype(np.float32), rng.standard_normal((2, 2, 3, 4, 1, 8)).astype(np.float32)
+        got = interp.run_text(text, [q, c, np.array([[2, 0]], np.int32), np.array([7], np.int32)])[0]
+        np.testing.assert_allclose(got, operators.paged_attention(q, c, np.array([[2, 0]]), [7], layer=1, window=5), rtol=1e-6)
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(H=7), "multiple of the number of key-value heads"), (dict(D=60), "multiple of 8"), (dict(D=264), "multiple of 8 from 8 to 256"),
+    (dict(layer=2), "layer"), (dict(window=-1), "window"), (dict(sinks=3), "sinks without a window"), (dict(dt="f64"), "f32, bf16 or f16"),
+    (dict(W=1 << 26, S=16), "2^30 positions"), (dict(scale=float("inf")), "no number"), (dict(L=0), "layer"), (dict(S=0), "one position"),
+])
+def test_paged_attention_refuses(kw, why):
+    with pytest.raises(b200.B200Error) as e:
+        b200.compile_to_plan(paged_text(**kw))
+    assert "b200.paged_attention" in str(e.value) and why in str(e.value)
+
+
+def refused(target, types, results, config=""):
+    names = [f"%arg{i}" for i in range(len(types))]
+    text = f"""module @jit_f {{
+  func.func public @main({", ".join(f"{n}: tensor<{t}>" for n, t in zip(names, types))}) -> (tensor<{results[0]}>) {{
+    %0:{len(results)} = "stablehlo.custom_call"({", ".join(names)}) <{{call_target_name = "{target}", backend_config = {{{config}}}}}> : ({", ".join(f"tensor<{t}>" for t in types)}) -> ({", ".join(f"tensor<{t}>" for t in results)})
+    "func.return"(%0#0) : (tensor<{results[0]}>) -> ()
+  }}
+}}"""
+    with pytest.raises(b200.B200Error) as e:
+        b200.compile_to_plan(text)
+    return str(e.value)
+
+
+def test_other_refusals():
+    paged = ["1x2x8xf32", "1x2x3x4x1x8xf32", "1x2xi32", "1xi32"]
+    assert "page table has to be" in refused("b200.paged_attention", [*paged[:2], "2x2xi32", paged[3]], ["1x2x8xf32"])
+    assert "lengths" in refused("b200.paged_attention", [*paged[:3], "1xi64"], ["1x2x8xf32"])
+    assert "the cache" in refused("b200.paged_attention", [paged[0], "1x2x3x4x1x8xbf16", *paged[2:]], ["1x2x8xf32"])
+    assert "the cache" in refused("b200.paged_attention", [paged[0], "1x3x3x4x1x8xf32", *paged[2:]], ["1x2x8xf32"])
+    assert "6 dimensions" in refused("b200.paged_attention", [paged[0], "1x2x3x4x8xf32", *paged[2:]], ["1x2x8xf32"])
+    assert "new keys" in refused("b200.paged_attention", [*paged, "1x2x1x8xf32"], ["1x2x8xf32"])
+    assert "result" in refused("b200.paged_attention", paged, ["1x2x8xbf16"])
+    assert "operands" in refused("b200.paged_attention", paged[:3], ["1x2x8xf32"])
+    assert "no attribute of this name: softcap" in refused("b200.paged_attention", paged, ["1x2x8xf32"], "softcap = 1 : i64")
+    assert "whole number" in refused("b200.paged_attention", paged, ["1x2x8xf32"], "window = 1.5 : f32")
+    prompt = ["2x5x4x8xf32", "2x5x2x8xf32", "2x5x2x8xf32"]
+    assert "v has to be" in refused("b200.window_attention", [*prompt[:2], "2x5x1x8xf32"], ["2x5x4x8xf32"])
+    assert "k has to be" in refused("b200.window_attention", [prompt[0], "2x6x2x8xf32", prompt[2]], ["2x5x4x8xf32"])
+    assert "multiple" in refused("b200.window_attention", [prompt[0], "2x5x3x8xf32", "2x5x3x8xf32"], ["2x5x4x8xf32"])
+    assert "alternatives" in refused("b200.token_log_probs", ["3x5xf32", "3xi32"], ["3xf32"] * 4 + ["3x6xf32", "3x6xi32"], "top = 6 : i64")
+    assert "from 0 to 128" in refused("b200.token_log_probs", ["3x500xf32", "3xi32"], ["3xf32"] * 4 + ["3x129xf32", "3x129xi32"], "top = 129 : i64")
+    assert "results" in refused("b200.token_log_probs", ["3x5xf32", "3xi32"], ["3xf32"] * 4, "top = 2 : i64")
+    assert "vocabulary is empty" in refused("b200.token_log_probs", ["3x0xf32", "3xi32"], ["3xf32"] * 4)
+    assert "tokens" in refused("b200.token_log_probs", ["3x5xf32", "4xi32"], ["3xf32"] * 4)
+    assert "not an operator" in refused("b200.decode_attention", paged, ["1x2x8xf32"])
+
+
+def test_gradient_of_token_log_probs_against_differences():
+    rng = np.random.default_rng(3)
+    x, t = rng.standard_normal((4, 9)) * 2, np.array([3, -1, 8, 0])
+    w = rng.standard_normal((3, 4))
+    f = lambda x: sum((a * b).sum() for a, b in zip(operators.token_log_probs(x, t), w))
+    dx = operators.token_log_probs_grad(x, t, *w)
+    for i in range(4):
+        for j in range(9):
+            e = np.zeros_like(x)
+            e[i, j] = 1e-5
+            # central differences: h^2 / 6 times a third derivative of order one, and rounding 1e-16 / h
+            assert abs((f(x + e) - f(x - e)) / 2e-5 - dx[i, j]) < 1e-8
+
+
+class HostClient:
+    """Stands in for a client: the cache is a NumPy array of one number per page and position."""
+
+    def __init__(self):
+        self.cache = None
+
+    def compile(self, text):
+        return self
+
+    def execute(self, args):
+        return [None]
+
+    def copy_pages(self, cache, pairs):
+        pairs = b200._indices(pairs, 2)
+        self.cache = operators.copy_pages(self.cache, pairs.tolist())
+
+    def write_pages(self, cache, rows, slots):
+        self.cache = operators.write_pages(self.cache, rows, b200._indices(slots, 1).tolist())
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_paged_cache_keeps_every_sequence(seed):
+    """Random growth, forks, ends and compactions: each sequence reads back the tokens that it was given, pages are never lost."""
+    rng = np.random.default_rng(seed)
+    size, pages = int(rng.integers(1, 5)), 24
+    host = HostClient()
+    cache = PagedCache(host, 1, pages, size, 1, 1)
+    host.cache = np.zeros((1, 2, pages, size, 1, 1))
+    want, token = {}, 1
+    for _ in range(300):
+        do = rng.integers(0, 10)
+        if do < 2 or not want:
+            want[cache.add()] = []
+        elif do < 6:
+            seqs = [s for s in want if rng.random() < 0.6]
+            counts = [int(rng.integers(0, 2 * size + 2)) for _ in seqs]
+            before = (cache.free_pages, [cache.lengths([s])[0] for s in seqs])
+            try:
+                slots = cache.extend(seqs, counts)
+            except b200.B200Error as e:
+                assert e.code == b200.RESOURCE_EXHAUSTED and before == (cache.free_pages, [cache.lengths([s])[0] for s in seqs])
+                continue
+            values = np.arange(token, token + len(slots), dtype=np.float64)
+            token += len(slots)
+            cache.write(values.reshape(1, 1, -1, 1, 1).repeat(2, 1), slots)
+            for s, n in zip(seqs, counts):
+                want[s] += values[:n].tolist()
+                values = values[n:]
+        elif do < 8:
+            s = list(want)[rng.integers(len(want))]
+            want[cache.fork(s)] = list(want[s])
+        elif do == 8:
+            s = list(want)[rng.integers(len(want))]
+            cache.free(s)
+            del want[s]
+        else:
+            cache.compact()
+            used = {p for s in want for p in cache.table([s])[0]}
+            assert used == set(range(len(used)))
+        for s, values in want.items():
+            table, n = cache.table([s], width=pages)[0], cache.lengths([s])[0]
+            assert n == len(values)
+            at = np.arange(n)
+            assert host.cache[0, 1, table[at // size], at % size, 0, 0].tolist() == values
+        assert cache.free_pages == pages - len({p for s in want for p in cache.table([s])[0]})
+
+
+def test_paged_cache_refuses():
+    host = HostClient()
+    cache = PagedCache(host, 1, 4, 2, 1, 1)
+    host.cache = np.zeros((1, 2, 4, 2, 1, 1))
+    s = cache.add()
+    for bad in (lambda: cache.extend([s, s], [1, 1]), lambda: cache.extend([s], [-1]), lambda: cache.extend([s], [1, 2]), lambda: cache.free(99),
+                lambda: cache.extend([99], [1]), lambda: PagedCache(host, 1, 0, 2, 1, 1), lambda: cache.lengths([5])):
+        with pytest.raises(b200.B200Error):
+            bad()
+    cache.extend([s], [5])
+    with pytest.raises(b200.B200Error):
+        cache.table([s], width=2)
+    with pytest.raises(b200.B200Error):
+        cache.extend([s], [4])
+    assert cache.free_pages == 1 and cache.lengths([s]).tolist() == [5]
+
+
+@pytest.mark.parametrize("values,ndim", [([[1, 2]], 1), ([1, 2], 2), ([[1, 2, 3]], 2), ([0.5], 1), ([2**31], 1), ([True], 1)])
+def test_indices_are_whole_numbers_of_32_bits(values, ndim):
+    with pytest.raises(b200.B200Error):
+        b200._indices(values, ndim)
