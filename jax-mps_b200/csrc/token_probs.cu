@@ -16,24 +16,26 @@ namespace b200 {
 namespace {
 
 struct Sums {
-  float m, s, u;
+  float m, s, u;                      // u in units of the logarithm to base 2
 };
+constexpr float kLowest = -3.4028235e38f;
+
+// 2^v; denormal results are zero.
+__device__ __forceinline__ float power(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Maxima start at the type's lowest value, not at minus infinity, so that differences with them are numbers; a side that has no
+// weight at the joint maximum adds nothing, however far below it is.
 __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == neg_inf()) return {m, a.s + b.s, a.u + b.u};
-  const float da = a.m - m, db = b.m - m, fa = __expf(da), fb = __expf(db);
-  // a side without weight adds nothing, however far it is below (its product with the distance could overflow)
+  const float m = fmaxf(a.m, b.m), da = (a.m - m) * kLog2e, db = (b.m - m) * kLog2e, fa = power(da), fb = power(db);
   return {m, fa * a.s + fb * b.s, (fa == 0.f ? 0.f : fa * (a.u + a.s * da)) + (fb == 0.f ? 0.f : fb * (b.u + b.s * db))};
 }
-template <typename F>
-__device__ __forceinline__ Sums block_join(Sums v, F* shared, int warps) {
+__device__ __forceinline__ Sums warp_join(Sums v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = join(v, {__shfl_xor_sync(0xFFFFFFFFu, v.m, o), __shfl_xor_sync(0xFFFFFFFFu, v.s, o), __shfl_xor_sync(0xFFFFFFFFu, v.u, o)});
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (lane == 0) shared[warp] = v;
-  __syncthreads();
-  v = shared[0];
-  for (int w = 1; w < warps; ++w) v = join(v, shared[w]);
   return v;
 }
 
@@ -44,58 +46,211 @@ __device__ __forceinline__ uint32_t order_of(float v) {
   return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
 
+constexpr int kThreads = 256, kWarps = kThreads / 32, kHeld = 32;      // logits that a thread holds
+constexpr int kSegment = kThreads * kHeld, kRoom = 1024, kMostTop = 128;
+constexpr int kNobody = 0x7FFFFFFF;
+
 struct Rows {
   const void* x;
   const int* tokens;
   float *log_prob, *entropy, *normalizer, *remainder, *top_values;
   int* top_ids;
-  int vocab, top;
+  Sums* sums;                         // of a row's segments, when there are several
+  uint2* best;                        // their `top` best as (order, number)
+  int vocab, top, segments;
+  long long rows;
 };
 
-// A block per row; the best alternatives one after another, each the first in order behind the one before.
+// The first `top` keys of a block in order, of those that its threads hold: N a thread, `order` with `id` (kNobody: none). Fewer
+// where there are fewer. `put(place, order, id)` gets each with its place. The top-th largest of the threads' own maxima is reached by
+// `top` keys at least, and for keys in no particular order by hardly more: it is found by a search over the key's bits, two at a time,
+// that ends when the number of maxima above is near enough. What reaches it is collected in shared memory and finds its place by
+// counting the keys in front of it, so that the result does not depend on the order of collection. More than there is room for (rows
+// of few distinct values): the search goes on over all keys, their numbers behind them, to the top-th itself.
+struct TopShared {
+  unsigned long long key[kRoom];
+  int total[64], found;
+};
+template <int N, typename Order, typename Id, typename Put>
+__device__ __forceinline__ void block_top(TopShared& sh, int top, Order&& order, Id&& id, Put&& put) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  if (tid < 64) sh.total[tid] = 0;
+  if (tid == 0) sh.found = 0;
+  uint32_t most = 0u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) { const uint32_t v = id(i) == kNobody ? 0u : order(i); most = v > most ? v : most; }
+  __syncthreads();
+  uint32_t least = 0u;
+  for (int b = 30, q = 0; b >= 0; b -= 2, q += 3) {
+#pragma unroll
+    for (int s = 1; s < 4; ++s) {
+      const uint32_t vote = __ballot_sync(0xFFFFFFFFu, most >= (least | ((uint32_t)s << b)));
+      if (lane == 0 && vote) atomicAdd(&sh.total[q + s - 1], __popc(vote));
+    }
+    __syncthreads();
+    int reached = kThreads;
+#pragma unroll
+    for (int s = 3; s > 0; --s)
+      if (sh.total[q + s - 1] >= top) { least |= (uint32_t)s << b; reached = sh.total[q + s - 1]; break; }
+    if (reached <= top + top / 2 + 8) break;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int j = id(i);
+    if (j != kNobody && order(i) >= least) {
+      const int at = atomicAdd(&sh.found, 1);
+      if (at < kRoom) sh.key[at] = (unsigned long long)order(i) << 32 | (0xFFFFFFFFu - (unsigned)j);
+    }
+  }
+  __syncthreads();
+  int count = sh.found;
+  if (count > kRoom) {
+    unsigned long long kth = 0;                               // the largest value that `top` keys reach
+    for (int b = 63; b >= 0; --b) {
+      const unsigned long long trial = kth | (1ull << b);
+      __syncthreads();
+      if (tid == 0) sh.found = 0;
+      __syncthreads();
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int j = id(i);
+        mine += j != kNobody && ((unsigned long long)order(i) << 32 | (0xFFFFFFFFu - (unsigned)j)) >= trial ? 1 : 0;
+      }
+      mine = __reduce_add_sync(0xFFFFFFFFu, mine);
+      if (lane == 0 && mine) atomicAdd(&sh.found, mine);
+      __syncthreads();
+      if (sh.found >= top) kth = trial;
+    }
+    __syncthreads();
+    if (tid == 0) sh.found = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int j = id(i);
+      const unsigned long long key = (unsigned long long)order(i) << 32 | (0xFFFFFFFFu - (unsigned)j);
+      if (j != kNobody && key >= kth) sh.key[atomicAdd(&sh.found, 1)] = key;
+    }
+    __syncthreads();
+    count = sh.found;                                         // `top`: no two keys are equal
+  }
+  for (int c = tid; c < count; c += kThreads) {
+    const unsigned long long key = sh.key[c];
+    int place = 0;
+    for (int o = 0; o < count; ++o) place += sh.key[o] > key ? 1 : 0;
+    if (place < top) put(place, (uint32_t)(key >> 32), (int)(0xFFFFFFFFu - (uint32_t)key));
+  }
+}
+
 template <typename T>
-__global__ void __launch_bounds__(256) probs_simple_kernel(const __grid_constant__ Rows a) {
+__device__ __forceinline__ void finish_row(const Rows& a, long long row, const Sums& v) {
+  // no weight at all: the logarithm of zero
+  const float ls = logf(v.s), n = v.s == 0.f ? neg_inf() : v.m + ls;
+  const int t = a.tokens[row];
+  a.log_prob[row] = t >= 0 && t < a.vocab ? (to_float(((const T*)a.x)[row * a.vocab + t]) - v.m) - ls + (v.s == 0.f ? n - n : 0.f) : 0.f;
+  a.entropy[row] = ls - v.u / v.s * kLn2;
+  a.normalizer[row] = n;
+  a.remainder[row] = (v.m - n) + ls;
+}
+template <typename T>
+__device__ __forceinline__ void finish_best(const Rows& a, long long row, const Sums& v, int place, int j) {
+  a.top_values[row * a.top + place] = (to_float(((const T*)a.x)[row * a.vocab + j]) - v.m) - logf(v.s);
+  a.top_ids[row * a.top + place] = j;
+}
+
+// A block takes a segment of a row, up to 8192 logits, which its threads hold: one pass over memory for the sums and the alternatives.
+// Pieces of 16 bytes that lie inside the row are read whole; rows need not begin at such a piece.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads) probs_kernel(const __grid_constant__ Rows a) {
   pdl_prologue();
-  __shared__ Sums shared[8];
-  __shared__ unsigned long long best[8];
-  const long long row = blockIdx.x;
+  constexpr int N = Pack<T>::N, NV = kHeld / N;
+  __shared__ Sums shared[kWarps];
+  __shared__ TopShared top;
+  const int tid = threadIdx.x, seg = (int)(blockIdx.x % a.segments);
+  const long long row = blockIdx.x / a.segments;
   const T* x = (const T*)a.x + row * a.vocab;
-  Sums v = {neg_inf(), 0.f, 0.f};
-  for (int j = threadIdx.x; j < a.vocab; j += 256) {
-    const float f = to_float(x[j]);
-    v = f == neg_inf() ? v : join(v, {f, 1.f, 0.f});
-    if (f != f) v.s = f;
-  }
-  v = block_join(v, shared, 8);
-  const float ls = logf(v.s), n = v.m + ls;
-  if (threadIdx.x == 0) {
-    const int t = a.tokens[row];
-    a.log_prob[row] = t >= 0 && t < a.vocab ? (to_float(x[t]) - v.m) - ls : 0.f;
-    a.entropy[row] = ls - v.u / v.s;
-    a.normalizer[row] = n;
-    a.remainder[row] = (v.m - n) + ls;
-  }
-  unsigned long long last = ~0ull;
-  for (int k = 0; k < a.top; ++k) {
-    unsigned long long mine = 0;
-    for (int j = threadIdx.x; j < a.vocab; j += 256) {
-      const unsigned long long key = (unsigned long long)order_of(to_float(x[j])) << 32 | (0xFFFFFFFFu - (unsigned)j);
-      if (key < last && key > mine) mine = key;
+  const int off = (int)(((unsigned long long)x / sizeof(T)) % N);     // logits of the row's first piece that belong to the row in front
+  const int pieces = (a.vocab + off + N - 1) / N, each = (pieces + a.segments - 1) / a.segments, p0 = seg * each, p1 = min(pieces, p0 + each);
+  float f[kHeld];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int p = p0 + tid + i * kThreads, j = p * N - off;
+    float g[N];
+    if (p < p1 && j >= 0 && j + N <= a.vocab) {
+      unpack<T>(__ldcs((const uint4*)(x + j)), g);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) g[e] = p < p1 && j + e >= 0 && j + e < a.vocab ? to_float(x[j + e]) : neg_inf();
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) { const unsigned long long w = __shfl_xor_sync(0xFFFFFFFFu, mine, o); mine = w > mine ? w : mine; }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) best[threadIdx.x >> 5] = mine;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; ++w) mine = best[w] > mine ? best[w] : mine;
-    last = mine;
-    const int j = (int)(0xFFFFFFFFu - (unsigned)mine);
-    if (threadIdx.x == 0) {
-      a.top_values[row * a.top + k] = (to_float(x[j]) - v.m) - ls;
-      a.top_ids[row * a.top + k] = j;
-    }
+    for (int e = 0; e < N; ++e) f[i * N + e] = g[e];
   }
+  Sums v = {kLowest, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) v.m = fmaxf(v.m, f[i]);
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const float t = (f[i] - v.m) * kLog2e, e = power(t);
+    v.s += e;
+    v.u = fmaf(e, fmaxf(t, -200.f), v.u);                             // the product of no weight and minus infinity is nothing
+  }
+  v = warp_join(v);
+  if ((tid & 31) == 0) shared[tid >> 5] = v;
+  __syncthreads();
+  v = shared[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) v = join(v, shared[w]);
+  const bool whole = a.segments == 1;
+  if (tid == 0) {
+    if (whole) finish_row<T>(a, row, v);
+    else a.sums[blockIdx.x] = v;
+  }
+  if (TOP) {
+    uint2* best = a.best + (long long)blockIdx.x * a.top;
+    const int have = max(0, min(a.top, min(a.vocab, p1 * N - off) - max(0, p0 * N - off)));
+    if (!whole && tid < a.top && tid >= have) best[tid] = make_uint2(0u, kNobody);
+    block_top<kHeld>(top, have, [&](int i) { return order_of(f[i]); },
+                     [&](int i) {
+                       const int p = p0 + tid + i / N * kThreads, j = p * N - off + i % N;
+                       return p < p1 && j >= 0 && j < a.vocab ? j : kNobody;
+                     },
+                     [&](int place, uint32_t order, int j) {
+                       if (whole) finish_best<T>(a, row, v, place, j);
+                       else best[place] = make_uint2(order, (unsigned)j);
+                     });
+  }
+}
+
+// Joins the segments of a row, in their order: a block per row where alternatives are wanted, else a warp.
+template <typename T>
+__device__ __forceinline__ Sums row_sums(const Rows& a, long long row) {
+  Sums v = {kLowest, 0.f, 0.f};
+  for (int i = threadIdx.x & 31; i < a.segments; i += 32) v = join(v, a.sums[row * a.segments + i]);
+  return warp_join(v);
+}
+template <typename T>
+__global__ void __launch_bounds__(kThreads) probs_join_kernel(const __grid_constant__ Rows a) {
+  pdl_prologue();
+  const long long row = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (row >= a.rows) return;
+  const Sums v = row_sums<T>(a, row);
+  if ((threadIdx.x & 31) == 0) finish_row<T>(a, row, v);
+}
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads) probs_join_top_kernel(const __grid_constant__ Rows a) {
+  pdl_prologue();
+  __shared__ TopShared top;
+  const long long row = blockIdx.x;
+  const Sums v = row_sums<T>(a, row);
+  if (threadIdx.x == 0) finish_row<T>(a, row, v);
+  uint2 held[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = threadIdx.x + i * kThreads;
+    held[i] = c < a.segments * a.top ? a.best[row * a.segments * a.top + c] : make_uint2(0u, kNobody);
+  }
+  block_top<N>(top, a.top, [&](int i) { return held[i].x; }, [&](int i) { return (int)held[i].y; },
+               [&](int place, uint32_t, int j) { finish_best<T>(a, row, v, place, j); });
 }
 
 struct Grad {
@@ -103,44 +258,91 @@ struct Grad {
   const int* tokens;
   const float *normalizer, *remainder, *entropy, *d_log_prob, *d_entropy, *d_normalizer;
   void* dx;
-  int vocab;
+  int vocab, segments;
 };
 
+// The same pieces of the logits and of their gradient, one after another: nothing is held.
 template <typename T>
-__global__ void __launch_bounds__(256) probs_grad_simple_kernel(const __grid_constant__ Grad a) {
+__global__ void __launch_bounds__(kThreads) probs_grad_kernel(const __grid_constant__ Grad a) {
   pdl_prologue();
-  const long long row = blockIdx.x;
+  constexpr int N = Pack<T>::N, NV = kHeld / N;
+  const int tid = threadIdx.x, seg = (int)(blockIdx.x % a.segments);
+  const long long row = blockIdx.x / a.segments;
   const T* x = (const T*)a.x + row * a.vocab;
   T* dx = (T*)a.dx + row * a.vocab;
+  const int off = (int)(((unsigned long long)x / sizeof(T)) % N);
+  const int pieces = (a.vocab + off + N - 1) / N, each = (pieces + a.segments - 1) / a.segments, p0 = seg * each, p1 = min(pieces, p0 + each);
   const int t = a.tokens[row];
   const float n = a.normalizer[row], low = a.remainder[row], h = a.entropy[row], dh = a.d_entropy[row], dl = t >= 0 && t < a.vocab ? a.d_log_prob[row] : 0.f;
   const float c = a.d_normalizer[row] - dl;
-  for (int j = threadIdx.x; j < a.vocab; j += 256) {
-    const float y = (to_float(x[j]) - n) - low, p = __expf(y);
-    const float e = p > 0.f ? p * (y + h) : p;
-    dx[j] = from_float<T>((j == t ? dl : 0.f) + p * c - dh * e);
+  auto value = [&](float v, int j) {
+    const float y = (v - n) - low, p = power(y * kLog2e);
+    return (j == t ? dl : 0.f) + p * (c - dh * (fmaxf(y, -200.f) + h));
+  };
+  uint4 held[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int p = p0 + tid + i * kThreads, j = p * N - off;
+    if (p < p1 && j >= 0 && j + N <= a.vocab) held[i] = __ldcs((const uint4*)(x + j));
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int p = p0 + tid + i * kThreads, j = p * N - off;
+    if (p >= p1) break;
+    if (j >= 0 && j + N <= a.vocab) {
+      float f[N];
+      unpack<T>(held[i], f);
+      uint4 out;
+      T* o = reinterpret_cast<T*>(&out);
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] = from_float<T>(value(f[e], j + e));
+      *(uint4*)(dx + j) = out;
+    } else {
+      for (int e = 0; e < N; ++e)
+        if (j + e >= 0 && j + e < a.vocab) dx[j + e] = from_float<T>(value(to_float(x[j + e]), j + e));
+    }
   }
 }
 
+// Segments of a row: as few as hold it (a first piece that starts in front of the row counts), and more for few rows, down to 2048
+// logits, so that the blocks fill the chip.
+int segments_of(const OperatorLaunch& op) {
+  const long long least = (op.vocab + 8 + kSegment - 1) / kSegment, most = std::max<long long>(least, op.vocab / 2048);
+  return (int)std::max<long long>(least, std::min<long long>(most, 2 * kSMs / std::max<long long>(1, op.rows)));
+}
+
 template <typename T>
-cudaError_t launch_rows(const Rows& a, long long rows, cudaStream_t stream, int* launches) {
-  return launch_op(probs_simple_kernel<T>, dim3((unsigned)rows), 256, 0, stream, launches, a);
+cudaError_t launch_rows(const Rows& a, cudaStream_t stream, int* launches) {
+  const dim3 grid((unsigned)(a.rows * a.segments));
+  if (cudaError_t e = a.top ? launch_op(probs_kernel<T, true>, grid, kThreads, 0, stream, launches, a) : launch_op(probs_kernel<T, false>, grid, kThreads, 0, stream, launches, a))
+    return e;
+  if (a.segments == 1) return cudaSuccess;
+  if (!a.top) return launch_op(probs_join_kernel<T>, dim3((unsigned)((a.rows + kWarps - 1) / kWarps)), kThreads, 0, stream, launches, a);
+  const int each = (a.segments * a.top + kThreads - 1) / kThreads;
+  if (each <= 4) return launch_op(probs_join_top_kernel<T, 4>, dim3((unsigned)a.rows), kThreads, 0, stream, launches, a);
+  if (each <= 16) return launch_op(probs_join_top_kernel<T, 16>, dim3((unsigned)a.rows), kThreads, 0, stream, launches, a);
+  return launch_op(probs_join_top_kernel<T, 64>, dim3((unsigned)a.rows), kThreads, 0, stream, launches, a);
 }
 template <typename T>
 cudaError_t launch_grad(const Grad& a, long long rows, cudaStream_t stream, int* launches) {
-  return launch_op(probs_grad_simple_kernel<T>, dim3((unsigned)rows), 256, 0, stream, launches, a);
+  return launch_op(probs_grad_kernel<T>, dim3((unsigned)(rows * a.segments)), kThreads, 0, stream, launches, a);
 }
 
 }  // namespace
 
 const char* token_log_probs_plan(OperatorLaunch& op) {
-  if (op.rows >= (1LL << 31)) return "2^31 rows and more";
-  op.scratch_bytes = 0;
-  op.launches = 1;
+  if (op.vocab > (1 << 30)) return "a vocabulary of more than 2^30";
+  const bool grad = op.kind == OperatorLaunch::TOKEN_LOG_PROBS_GRAD;
+  int s = segments_of(op);
+  if (op.top && (long long)s * op.top > 64 * kThreads) return "more alternatives than this vocabulary's segments leave room for";
+  if (op.rows * s >= (1LL << 31)) return "too many logits";
+  const bool several = !grad && s > 1;
+  op.scratch_bytes = several ? op.rows * s * (12 + 8LL * op.top) + 16 : 0;
+  op.launches = several ? 2 : 1;
   return nullptr;
 }
 
-cudaError_t launch_token_log_probs(const OperatorLaunch& op, void* const* args, void*, cudaStream_t stream, int* launches) {
+cudaError_t launch_token_log_probs(const OperatorLaunch& op, void* const* args, void* scratch, cudaStream_t stream, int* launches) {
   Rows a = {};
   const int results = op.top ? 6 : 4;
   a.log_prob = (float*)args[0];
@@ -152,9 +354,13 @@ cudaError_t launch_token_log_probs(const OperatorLaunch& op, void* const* args, 
   a.tokens = (const int*)args[results + 1];
   a.vocab = op.vocab;
   a.top = op.top;
-  if (op.type == 0) return launch_rows<float>(a, op.rows, stream, launches);
-  if (op.type == 1) return launch_rows<__nv_bfloat16>(a, op.rows, stream, launches);
-  return launch_rows<__half>(a, op.rows, stream, launches);
+  a.rows = op.rows;
+  a.segments = segments_of(op);
+  a.best = (uint2*)scratch;
+  a.sums = (Sums*)((char*)scratch + op.rows * a.segments * 8LL * op.top);
+  if (op.type == 0) return launch_rows<float>(a, stream, launches);
+  if (op.type == 1) return launch_rows<__nv_bfloat16>(a, stream, launches);
+  return launch_rows<__half>(a, stream, launches);
 }
 
 cudaError_t launch_token_log_probs_grad(const OperatorLaunch& op, void* const* args, cudaStream_t stream, int* launches) {
@@ -169,6 +375,7 @@ cudaError_t launch_token_log_probs_grad(const OperatorLaunch& op, void* const* a
   a.d_entropy = (const float*)args[7];
   a.d_normalizer = (const float*)args[8];
   a.vocab = op.vocab;
+  a.segments = segments_of(op);
   if (op.type == 0) return launch_grad<float>(a, op.rows, stream, launches);
   if (op.type == 1) return launch_grad<__nv_bfloat16>(a, op.rows, stream, launches);
   return launch_grad<__half>(a, op.rows, stream, launches);
