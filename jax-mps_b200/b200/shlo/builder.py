@@ -840,7 +840,7 @@ class Builder:
         the pages of each sequence in order, `lengths` i32[batch] how many positions of them are filled. Query head h reads
         key-value head h // (heads / kv_heads). `new` [2, batch, kv_heads, head_dim] is the token's own key and value, which are not in
         the cache yet: the token stands at position lengths[b] then, otherwise at lengths[b] - 1, the last cached one. With a
-        `window`, position j is visible from p when p - j < window or j < sinks. `scale` is 1 / sqrt(head_dim) by default. A
+        `window`, position j is visible from p when p - j < window or j < sinks. `scale`, above zero, is 1 / sqrt(head_dim) by default. A
         sequence that sees nothing gives zeros; lengths below zero count as zero and above the table's room as that; pages
         that the table names outside the cache are left out. f32, bf16 or f16, sums in 32 bits. No gradient."""
         xs = [q, cache, table, lengths] + ([new] if new is not None else [])

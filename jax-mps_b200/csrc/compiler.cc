@@ -2919,6 +2919,7 @@ struct Planner {
       if (h < 1 || kv < 1 || h % kv) fail("the number of query heads (" + std::to_string(h) + ") has to be a multiple of the number of key-value heads (" + std::to_string(kv) + ")");
       if (d < 8 || d > 256 || d % 8) fail("head features have to be a multiple of 8 from 8 to 256, got " + std::to_string(d));
       o.scale = (float)number("scale", 1.0 / std::sqrt((double)d));
+      if (!(o.scale > 0.f) || !std::isfinite(o.scale)) fail("the scale has to be positive and finite in 32 bits");
       o.window = (int)whole("window", 0, 0, (1LL << 30));
       o.sinks = (int)whole("sinks", 0, 0, (1LL << 30));
       if (o.sinks && !o.window) fail("sinks without a window");

@@ -53,7 +53,7 @@ def test_the_assembly_jax_prints():
 @pytest.mark.parametrize("kw,why", [
     (dict(H=7), "multiple of the number of key-value heads"), (dict(D=60), "multiple of 8"), (dict(D=264), "multiple of 8 from 8 to 256"),
     (dict(layer=2), "layer"), (dict(window=-1), "window"), (dict(sinks=3), "sinks without a window"), (dict(dt="f64"), "f32, bf16 or f16"),
-    (dict(W=1 << 26, S=16), "2^30 positions"), (dict(scale=float("inf")), "no number"), (dict(L=0), "layer"), (dict(S=0), "one position"),
+    (dict(W=1 << 26, S=16), "2^30 positions"), (dict(scale=float("inf")), "no number"), (dict(scale=-0.5), "positive"), (dict(scale=0.0), "positive"), (dict(scale=1e300), "positive"), (dict(L=0), "layer"), (dict(S=0), "one position"),
 ])
 def test_paged_attention_refuses(kw, why):
     with pytest.raises(b200.B200Error) as e:
