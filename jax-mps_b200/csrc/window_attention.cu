@@ -165,7 +165,8 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const __grid_constant__
 // copies into 128-byte-swizzled shared memory, warp 5 issues tcgen05.mma: scores = Q K^T from shared memory into tensor memory, then
 // O += P V with the weights P read from tensor memory, where they take the place of the scores. Warps 0-3 hold a row a thread: they
 // read the scores, mask them, exponentiate and round the weights to 16 bits (the one rounding beside the result's: the second
-// product's operands have 16 bits), and keep maximum and sum. The outputs are scaled to a new maximum only when it has grown by more
+// product's operands have 16 bits), and keep maximum and sum; the first half of a tile's weights is multiplied while the second is
+// made. The outputs are scaled to a new maximum only when it has grown by more
 // than 2^8 since the last time; the weights are at most 2^8 until then, which no type minds, and the sums are divided in the end by
 // a sum that was taken in the same units. Heads of up to 128 features: two blocks an SM, so that one's products run while the other
 // exponentiates. Heads of up to 256: one block, and two tiles of scores in tensor memory.
@@ -211,27 +212,20 @@ __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::afte
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 32 columns of a thread's lane of tensor memory; the wait belongs to the load, so that no use comes before it.
+// 32 columns of a thread's lane of tensor memory. Loads are on their way until `loaded` has been passed, and what they give is touched by
+// `settle` behind it, so that no use of it can come before.
 __device__ __forceinline__ void load32(uint32_t addr, uint32_t* v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
-      "%24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
-        "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
-        "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(addr)
-      : "memory");
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+               : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void settle(uint32_t* v) {
+  asm volatile("" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
 }
 __device__ __forceinline__ void store32(uint32_t addr, const uint32_t* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, "
-      "%25, %26, %27, %28, %29, %30, %31, %32};"
-      ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
-        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
-        "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+               ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pair16(float lo, float hi) {
@@ -243,6 +237,27 @@ __device__ __forceinline__ uint32_t pair16(float lo, float hi) {
 __device__ __forceinline__ float power(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two floats in a register pair, for the instructions that take both at once.
+__device__ __forceinline__ uint64_t two(uint32_t x, uint32_t y) { return (uint64_t)y << 32 | x; }
+__device__ __forceinline__ uint64_t two(float x, float y) { return two(__float_as_uint(x), __float_as_uint(y)); }
+__device__ __forceinline__ float first(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float second(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 
@@ -280,8 +295,8 @@ __global__ void __launch_bounds__(kMmaThreads, Mma<DP>::BLOCKS_PER_SM) prompt_mm
   uint8_t *qs = smem, *ks = qs + C::TILE, *vs = ks + S * C::TILE;
   uint64_t* bars = (uint64_t*)(vs + S * C::TILE);
   const uint32_t q_full = smem_u32(bars), k_full = q_full + 8, k_empty = k_full + 8 * S, v_full = k_empty + 8 * S, v_empty = v_full + 8 * S,
-                 s_full = v_empty + 8 * S, p_full = s_full + 8 * NS, pv_done = p_full + 8 * NS, drained = pv_done + 8;
-  uint32_t* tmem_slot = (uint32_t*)(bars + 3 + 4 * S + 2 * NS);
+                 s_full = v_empty + 8 * S, p_full = s_full + 8 * NS, pv_done = p_full + 16 * NS, drained = pv_done + 8;
+  uint32_t* tmem_slot = (uint32_t*)(bars + 3 + 4 * S + 3 * NS);
   volatile int* failed = (volatile int*)(tmem_slot + 1);
   if (tid == 0) {
     for (uint32_t bar = q_full; bar <= drained; bar += 8) mbar_init(bar, bar >= p_full && bar < pv_done ? 4 : 1);
@@ -370,15 +385,20 @@ __global__ void __launch_bounds__(kMmaThreads, Mma<DP>::BLOCKS_PER_SM) prompt_mm
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
-      wait(p_full + 8 * (i % NS), (i / NS) & 1);
-      if (ok && elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < kRows / 16; ++kk)
-          mma_tmem(t_out, tmem + i % NS * kRows + kk * 8, d_v + (uint64_t)((s * C::TILE + kk * 2048) >> 4), idesc_o, i > 0 || kk > 0);
-        commit(v_empty + 8 * s);
-        commit(pv_done);
+      for (int half = 0; half < 2; ++half) {
+        wait(p_full + 16 * (i % NS) + 8 * half, (i / NS) & 1);
+        if (ok && elect_one()) {
+#pragma unroll
+          for (int kk = half * (kRows / 32); kk < (half + 1) * (kRows / 32); ++kk)
+            mma_tmem(t_out, tmem + i % NS * kRows + kk * 8, d_v + (uint64_t)((s * C::TILE + kk * 2048) >> 4), idesc_o, i > 0 || kk > 0);
+          if (half) {
+            commit(v_empty + 8 * s);
+            commit(pv_done);
+          }
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
     if (!ok || *failed) {                                            // tensor memory goes back only when no product is left
       if (elect_one()) commit(drained);
@@ -405,16 +425,32 @@ __global__ void __launch_bounds__(kMmaThreads, Mma<DP>::BLOCKS_PER_SM) prompt_mm
       uint32_t s[kRows];
 #pragma unroll
       for (int c = 0; c < kRows; c += 32) load32(t_s + c, s + c);
-      if (!(k0 + kRows - 1 <= q0 && (a.window == 0 || q0 + kRows - 1 - k0 < a.window || k0 + kRows <= a.sinks))) {
-        const int most = row - k0, least = a.window > 0 ? row - a.window + 1 - k0 : 0, always = a.sinks - k0;
+      loaded();
+#pragma unroll
+      for (int c = 0; c < kRows; c += 32) settle(s + c);
+      // masks at the edges only: the last key that the row sees, the first of its window, the sinks
+      const bool late = k0 + kRows - 1 > q0, early = a.window > 0 && q0 + kRows - 1 - k0 >= a.window && k0 + kRows > a.sinks;
+      if (early && k0 < a.sinks) {
+        const int least = row - a.window + 1 - k0, always = a.sinks - k0;
 #pragma unroll
         for (int k = 0; k < kRows; ++k)
-          if (k > most || (k < least && k >= always)) s[k] = 0xFF800000u;
+          if (k < least && k >= always) s[k] = 0xFF800000u;
+      } else if (early) {
+        const int least = row - a.window + 1 - k0;
+#pragma unroll
+        for (int k = 0; k < kRows; ++k)
+          if (k < least) s[k] = 0xFF800000u;
+      }
+      if (late) {
+        const int most = row - k0;
+#pragma unroll
+        for (int k = 0; k < kRows; ++k)
+          if (k > most) s[k] = 0xFF800000u;
       }
       float top[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
 #pragma unroll
-      for (int k = 0; k < kRows; ++k) top[k % 4] = fmaxf(top[k % 4], __uint_as_float(s[k]));
-      const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      for (int k = 0; k < kRows; k += 2) top[k / 2 % 4] = max3(top[k / 2 % 4], __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+      const float best = fmaxf(max3(top[0], top[1], top[2]), top[3]);
       const bool grown = best > m && (best - m) * a.scale > kGrowth;
       if (__any_sync(0xFFFFFFFFu, grown)) {
         const float now = fmaxf(m, best), keep = m == neg_inf() ? 0.f : power((m - now) * a.scale);
@@ -422,10 +458,12 @@ __global__ void __launch_bounds__(kMmaThreads, Mma<DP>::BLOCKS_PER_SM) prompt_mm
         l *= keep;
         if (i > 0) {
           if (!wait(pv_done, (i - 1) & 1)) break;
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < DP; c += 32) {
             uint32_t o[32];
             load32(t_out + mine + c, o);
+            loaded();
+            settle(o);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
             store32(t_out + mine + c, o);
@@ -433,20 +471,26 @@ __global__ void __launch_bounds__(kMmaThreads, Mma<DP>::BLOCKS_PER_SM) prompt_mm
         }
       }
       const float ref = m == neg_inf() ? 0.f : m * a.scale - shift;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t scale = two(a.scale, a.scale), minus = two(-ref, -ref);
+      uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int k = 0; k < kRows; k += 2) {
-        const float x = power(fmaf(__uint_as_float(s[k]), a.scale, -ref)), y = power(fmaf(__uint_as_float(s[k + 1]), a.scale, -ref));
-        sum[k / 2 % 4] += x + y;
-        s[k / 2] = pair16<T>(x, y);
+      for (int half = 0; half < 2; ++half) {
+        uint32_t p[32];
+#pragma unroll
+        for (int k = 0; k < kRows / 2; k += 2) {
+          const uint64_t x = fma2(two(s[half * (kRows / 2) + k], s[half * (kRows / 2) + k + 1]), scale, minus);
+          const float a0 = power(first(x)), a1 = power(second(x));
+          sum[k / 2 % 4] = add2(sum[k / 2 % 4], two(a0, a1));
+          p[k / 2] = pair16<T>(a0, a1);
+        }
+        store32(t_s + half * 32, p);
+        stored();
+        before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + 16 * (i % NS) + 8 * half);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      store32(t_s, s);
-      store32(t_s + 32, s + 32);
-      stored();
-      before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + 8 * (i % NS));
+      const uint64_t all = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+      l += first(all) + second(all);
     }
     if (ok && wait(pv_done, (tiles.count - 1) & 1)) {
       const bool some = row < n;
@@ -455,6 +499,8 @@ __global__ void __launch_bounds__(kMmaThreads, Mma<DP>::BLOCKS_PER_SM) prompt_mm
       for (int c = 0; c < DP; c += 32) {
         uint32_t o[32];
         load32(t_out + mine + c, o);
+        loaded();
+        settle(o);
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
           if (row < a.tokens && c + e < D) {
