@@ -21,6 +21,8 @@ struct Prompt {
   void* out;
   int batch, tokens, heads, kv_heads, dim, group, window, sinks;
   float scale;                        // of the scores, times log2(e)
+  // tensor cores: whether a block's two tiles of queries are two heads (else two tiles of one), units of heads and of queries, all units
+  int pairs, head_units, query_units, units;
 };
 
 __device__ __forceinline__ int length_of(const Prompt& a, int b) {
@@ -161,26 +163,33 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const __grid_constant__
 }
 
 // ---- 16-bit data on the tensor cores -------------------------------------------------------------------
-// A block takes 128 queries of a head in tiles of 128 keys. Warp 4 brings the queries and the tiles of keys and values by TMA tiled
-// copies into 128-byte-swizzled shared memory, warp 5 issues tcgen05.mma: scores = Q K^T from shared memory into tensor memory, then
-// O += P V with the weights P read from tensor memory, where they take the place of the scores. Warps 0-3 hold a row a thread: they
-// read the scores, mask them, exponentiate and round the weights to 16 bits (the one rounding beside the result's: the second
-// product's operands have 16 bits), and keep maximum and sum; the first half of a tile's weights is multiplied while the second is
-// made. The outputs are scaled to a new maximum only when it has grown by more
-// than 2^8 since the last time; the weights are at most 2^8 until then, which no type minds, and the sums are divided in the end by
-// a sum that was taken in the same units. Heads of up to 128 features: two blocks an SM, so that one's products run while the other
-// exponentiates. Heads of up to 256: one block, and two tiles of scores in tensor memory.
-constexpr int kRows = 128, kMmaThreads = 192;
+// A block, one per SM, goes from one tile of 128 queries of a head to another, or takes two of them along that read the same keys: two
+// heads that share a key-value head, or two tiles of one head. Warp 8 brings queries and tiles of 128 keys and values by TMA tiled
+// copies into 128-byte-swizzled shared memory, a tile or more ahead of warp 9, which issues tcgen05.mma: scores = Q K^T from shared
+// memory into tensor memory, then O += P V with the weights P read from tensor memory, where they take the place of the scores.
+// Warps 0-7 read the scores, mask them, exponentiate and round the weights to 16 bits (the one rounding beside the result's: the second
+// product's operands have 16 bits): four for each tile of queries, a thread a row, or with one tile two threads a row, which agree on
+// its maximum. One tile's products run while the other's weights are made; a single tile has two places for its scores instead. The
+// first half of a row's weights is multiplied while the second is made. The outputs are scaled to a new maximum only when it has
+// grown by more than 2^8 since the last time; the weights are at most 2^8 until then, which no type minds, and the sums are divided
+// in the end by a sum that was taken in the same units.
+// Products of a block run in the order in which its one thread issued them, so that scores may go where the weights of a product in
+// front are read.
+constexpr int kRows = 128, kMmaThreads = 320;
 constexpr float kGrowth = 8.f;
+constexpr int kByFma = 0;             // of eight pairs of exponentials, how many the FMA pipe makes
 
-template <int DP>
+constexpr int kStagePitch = 80;       // bytes between rows of 32 results on their way out
+
+template <int DP, int ITEMS>
 struct Mma {
   static constexpr int BLOCKS = DP / 64, BLOCK = kRows * 128, TILE = BLOCKS * BLOCK;      // bytes: a box of 64 features, a tile
-  static constexpr int STAGES = DP == 64 ? 2 : 1;
-  static constexpr int SCORES = DP == 256 ? 2 : 1;                   // tiles of scores in tensor memory
-  static constexpr int COLUMNS = DP == 256 ? 512 : 256;
-  static constexpr int BLOCKS_PER_SM = DP == 256 ? 1 : 2;
-  static constexpr int SMEM = TILE * (1 + 2 * STAGES) + 1024 + 256;
+  static constexpr int STAGES = DP == 64 ? 4 : DP == 128 ? 2 : 1;
+  static constexpr int HALVES = ITEMS == 1 ? 2 : 1, COLS = kRows / HALVES;               // threads of a row, scores of a thread
+  static constexpr int SMEM = TILE * (ITEMS + 2 * STAGES) + 1024 + 512 + 4 * kRows * 4 + 8 * 32 * kStagePitch;
+  static_assert(SMEM <= 232448, "more than an SM has");
+  // columns of the weights of one half of a tile's keys: over the scores of the thread that makes them
+  static __device__ __forceinline__ int weights(int half) { return half * (ITEMS == 2 ? 32 : 64); }
 };
 
 __device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
@@ -223,6 +232,14 @@ __device__ __forceinline__ void loaded() { asm volatile("tcgen05.wait::ld.sync.a
 __device__ __forceinline__ void settle(uint32_t* v) {
   asm volatile("" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
 }
+// Eight columns scaled in place.
+__device__ __forceinline__ void scale8(uint32_t addr, float by) {
+  uint32_t v[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(addr) : "memory");
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * by);
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
 __device__ __forceinline__ void store32(uint32_t addr, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
                ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
@@ -245,6 +262,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 // Two floats in a register pair, for the instructions that take both at once.
 __device__ __forceinline__ uint64_t two(uint32_t x, uint32_t y) { return (uint64_t)y << 32 | x; }
 __device__ __forceinline__ uint64_t two(float x, float y) { return two(__float_as_uint(x), __float_as_uint(y)); }
@@ -261,266 +283,393 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// The tiles of keys that a tile of queries visits: those of the sinks in front of the window, then the window's.
-struct Tiles {
-  int sinks, first, count;
-  __device__ __forceinline__ Tiles(const Prompt& a, int q0, int n) {
-    first = a.window > 0 ? max(0, q0 - a.window + 1) / kRows : 0;
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x for two values on the FMA pipe, which has time while the one that does exponentials has none: x = n + f with n whole and f from -1/2
+// to 1/2, 2^f by the polynomial of degree three with the least relative error there (weighted least squares, weights repeated until
+// the error is even: 7.5e-5, 2^-5 of the 16-bit rounding that follows, 2^-2.7 of f16's), times 2^n. For x up to 127; NaN stays NaN.
+__device__ __forceinline__ uint64_t power2_by_fma(uint64_t x) {
+  constexpr float magic = 12582912.f;                                // 1.5 * 2^23: added, it leaves the whole part in the last bits
+  x = two(max_or_nan(first(x), -126.f), max_or_nan(second(x), -126.f));
+  const uint64_t t = add2(x, two(magic, magic)), f = add2(x, fma2(t, two(-1.f, -1.f), two(magic, magic)));
+  uint64_t r = fma2(two(0.05517166935952265f, 0.05517166935952265f), f, two(0.24261113138277257f, 0.24261113138277257f));
+  r = fma2(r, f, two(0.6932609862029611f, 0.6932609862029611f));
+  r = fma2(r, f, two(0.9999280729973529f, 0.9999280729973529f));
+  return mul2(r, two(((uint32_t)t << 23) + 0x3F800000u, ((uint32_t)(t >> 32) << 23) + 0x3F800000u));
+}
+
+// What a block does next: its tiles of queries and the tiles of keys that they visit, those of the sinks in front of the window, then
+// the window's.
+template <int ITEMS>
+struct Unit {
+  int b, kvh, n, first, sinks, count;
+  int head[ITEMS], q0[ITEMS];
+  __device__ __forceinline__ Unit(const Prompt& a, int unit) {
+    const int each = a.head_units * a.batch, rest = unit % each, hu = rest % a.head_units;
+    const int qu = a.query_units - 1 - unit / each;                  // the rows that see most go first
+    b = rest / a.head_units;
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+      head[u] = ITEMS == 2 && a.pairs ? hu * 2 + u : hu;
+      q0[u] = (ITEMS == 2 && !a.pairs ? qu * 2 + u : qu) * kRows;
+    }
+    kvh = head[0] / a.group;
+    n = length_of(a, b);
+    first = a.window > 0 ? max(0, q0[0] - a.window + 1) / kRows : 0;
     sinks = min((int)(((long long)a.sinks + kRows - 1) / kRows), first);
-    count = sinks + (min(q0 + kRows, n) - 1) / kRows - first + 1;
+    count = q0[0] >= n ? 0 : sinks + (min(q0[ITEMS - 1] + kRows, n) - 1) / kRows - first + 1;
   }
   __device__ __forceinline__ int key(int i) const { return (i < sinks ? i : first + i - sinks) * kRows; }
 };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kMmaThreads, Mma<DP>::BLOCKS_PER_SM) prompt_mma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                                                                                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Prompt a,
-                                                                                        int* __restrict__ error_flag) {
-  using C = Mma<DP>;
-  constexpr int S = C::STAGES, NS = C::SCORES, AHEAD = NS - 1;
-  pdl_prologue();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int h = blockIdx.x, b = blockIdx.z, kvh = h / a.group, n = length_of(a, b), D = a.dim;
-  const int q0 = (int)(gridDim.y - 1 - blockIdx.y) * kRows;          // the rows that see most go first
-  T* out = (T*)a.out + (((long long)b * a.tokens + q0) * a.heads + h) * D;
-  const long long pitch = (long long)a.heads * D;
-  if (q0 >= n) {
-    const uint4 zero = {0, 0, 0, 0};
-    for (int i = tid; i < kRows * (D / 8); i += kMmaThreads)
-      if (q0 + i / (D / 8) < a.tokens) *(uint4*)(out + i / (D / 8) * pitch + i % (D / 8) * 8) = zero;
-    return;
-  }
+template <typename T, int DP, int ITEMS>
+__global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                                                                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Prompt a,
+                                                                    int* __restrict__ error_flag) {
+  using C = Mma<DP, ITEMS>;
+  constexpr int S = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t *qs = smem, *ks = qs + C::TILE, *vs = ks + S * C::TILE;
+  uint8_t *qs = smem, *ks = qs + ITEMS * C::TILE, *vs = ks + S * C::TILE;
   uint64_t* bars = (uint64_t*)(vs + S * C::TILE);
-  const uint32_t q_full = smem_u32(bars), k_full = q_full + 8, k_empty = k_full + 8 * S, v_full = k_empty + 8 * S, v_empty = v_full + 8 * S,
-                 s_full = v_empty + 8 * S, p_full = s_full + 8 * NS, pv_done = p_full + 16 * NS, drained = pv_done + 8;
-  uint32_t* tmem_slot = (uint32_t*)(bars + 3 + 4 * S + 3 * NS);
+  // queries are there, are done with; keys and values likewise, a stage each; scores of a place; weights of a place, two halves; outputs
+  // of a tile have all products so far, have been read; both threads of a row have spoken; nothing is under way
+  constexpr int Q_FULL = 0, Q_EMPTY = 1, K_FULL = 2, K_EMPTY = K_FULL + S, V_FULL = K_EMPTY + S, V_EMPTY = V_FULL + S, S_FULL = V_EMPTY + S, P_FULL = S_FULL + 2,
+                PV_DONE = P_FULL + 4, O_EMPTY = PV_DONE + 2, AGREED = O_EMPTY + 2, DRAINED = AGREED + 4, BARRIERS = DRAINED + 1;
+  static_assert(BARRIERS * 8 + 8 <= 512, "barriers");
+  auto bar = [base = smem_u32(bars)](int k) { return base + 8u * (uint32_t)k; };
+  uint32_t* tmem_slot = (uint32_t*)(bars + BARRIERS);
   volatile int* failed = (volatile int*)(tmem_slot + 1);
+  float* said = (float*)((uint8_t*)bars + 512);                      // [parity][half][row]
+  uint8_t* stage = (uint8_t*)(said + 4 * kRows);                     // [warp][row][32 results]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, D = a.dim;
   if (tid == 0) {
-    for (uint32_t bar = q_full; bar <= drained; bar += 8) mbar_init(bar, bar >= p_full && bar < pv_done ? 4 : 1);
+    for (int k = 0; k < BARRIERS; ++k)
+      mbar_init(bar(k), k >= P_FULL && k < PV_DONE ? 4 : k >= O_EMPTY && k < AGREED ? 8 / ITEMS : k >= AGREED && k < DRAINED ? 2 : 1);
     *failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 5) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::COLUMNS) : "memory");
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   before_sync();
   __syncthreads();
   after_sync();
-  const uint32_t tmem = *tmem_slot, t_out = tmem + NS * kRows;
-  const Tiles tiles(a, q0, n);
+  const uint32_t tmem = *tmem_slot;
+  pdl_prologue();
+  // the place of a tile's scores and how often it has been used, by the number of the tile since the block began
+  auto place = [](int u, int it) { return ITEMS == 2 ? u : it & 1; };
+  auto turn = [](int it) { return ITEMS == 2 ? it & 1 : it >> 1 & 1; };
+  auto outputs = [&](int u) { return tmem + 256 + u * DP; };
 
-  if (warp == 4) {
+  if (warp == 8) {
     // ------------------------------ copies (one lane) -----------------------------------------------------------
     if (lane == 0) {
       bool ok = true;
-      int kt = 0, vt = 0;
-      const int row = b * a.tokens;
-      expect_bytes(q_full, C::TILE);
+      int it = 0, kt = 0, vt = 0, done = 0;
+      for (int unit = blockIdx.x; unit < a.units && ok; unit += gridDim.x) {
+        const Unit<ITEMS> w(a, unit);
+        if (!w.count) continue;
+        const int row = w.b * a.tokens;
+        if (done && !(ok = role_wait(bar(Q_EMPTY), (done - 1) & 1, failed))) break;
+        expect_bytes(bar(Q_FULL), ITEMS * C::TILE);
 #pragma unroll
-      for (int c = 0; c < C::BLOCKS; ++c) copy_box(smem_u32(qs) + c * C::BLOCK, &tm_q, q_full, c * 64, row + q0, h);
-      for (int i = 0; i < tiles.count; ++i) {
-        const int s = i % S, parity = ((i / S) & 1) ^ 1, k0 = row + tiles.key(i);
-        if (i >= S && !(ok = role_wait(k_empty + 8 * s, parity, failed))) break;
-        expect_bytes(k_full + 8 * s, C::TILE);
+        for (int u = 0; u < ITEMS; ++u)
 #pragma unroll
-        for (int c = 0; c < C::BLOCKS; ++c) copy_box(smem_u32(ks) + s * C::TILE + c * C::BLOCK, &tm_k, k_full + 8 * s, c * 64, k0, kvh);
-        ++kt;
-        if (i >= S && !(ok = role_wait(v_empty + 8 * s, parity, failed))) break;
-        expect_bytes(v_full + 8 * s, C::TILE);
+          for (int c = 0; c < C::BLOCKS; ++c) copy_box(smem_u32(qs) + u * C::TILE + c * C::BLOCK, &tm_q, bar(Q_FULL), c * 64, row + w.q0[u], w.head[u]);
+        ++done;
+        for (int i = 0; i < w.count; ++i, ++it) {
+          const int s = it % S, parity = ((it / S) & 1) ^ 1, k0 = row + w.key(i);
+          if (it >= S && !(ok = role_wait(bar(K_EMPTY + s), parity, failed))) break;
+          expect_bytes(bar(K_FULL + s), C::TILE);
 #pragma unroll
-        for (int c = 0; c < C::BLOCKS; ++c) copy_box(smem_u32(vs) + s * C::TILE + c * C::BLOCK, &tm_v, v_full + 8 * s, c * 64, k0, kvh);
-        ++vt;
+          for (int c = 0; c < C::BLOCKS; ++c) copy_box(smem_u32(ks) + s * C::TILE + c * C::BLOCK, &tm_k, bar(K_FULL + s), c * 64, k0, w.kvh);
+          ++kt;
+          if (it >= S && !(ok = role_wait(bar(V_EMPTY + s), parity, failed))) break;
+          expect_bytes(bar(V_FULL + s), C::TILE);
+#pragma unroll
+          for (int c = 0; c < C::BLOCKS; ++c) copy_box(smem_u32(vs) + s * C::TILE + c * C::BLOCK, &tm_v, bar(V_FULL + s), c * 64, k0, w.kvh);
+          ++vt;
+        }
       }
       if (!ok || *failed) {
         // copies that nobody consumed any more: wait for them before the shared memory goes away
-        mbar_wait(q_full, 0);
-        for (int j = max(0, kt - S); j < kt; ++j) mbar_wait(k_full + 8 * (j % S), (j / S) & 1);
-        for (int j = max(0, vt - S); j < vt; ++j) mbar_wait(v_full + 8 * (j % S), (j / S) & 1);
+        if (done) mbar_wait(bar(Q_FULL), (done - 1) & 1);
+        for (int j = max(0, kt - S); j < kt; ++j) mbar_wait(bar(K_FULL + j % S), (j / S) & 1);
+        for (int j = max(0, vt - S); j < vt; ++j) mbar_wait(bar(V_FULL + j % S), (j / S) & 1);
       }
     }
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     // ------------------------------ products --------------------------------------------------------------------
     constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     constexpr uint32_t common = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kRows >> 4) << 24);
     constexpr uint32_t idesc_s = common | ((uint32_t)(kRows >> 3) << 17), idesc_o = common | (1u << 16) | ((uint32_t)(DP >> 3) << 17);
     const uint64_t d_q = umma_desc(smem_u32(qs)), d_k = umma_desc(smem_u32(ks)), d_v = values_desc(smem_u32(vs));
     bool ok = true;
-    auto wait = [&](uint32_t bar, int parity) {
-      ok = __all_sync(0xFFFFFFFFu, ok && role_wait(bar, parity, failed));
+    auto wait = [&](int k, int parity) {
+      ok = __all_sync(0xFFFFFFFFu, ok && role_wait(bar(k), parity, failed));
       after_sync();
     };
-    auto scores = [&](int i) {
-      const int s = i % S;
-      wait(k_full + 8 * s, (i / S) & 1);
-      if (i >= NS) wait(pv_done, (i - NS) & 1);                       // the weights in this place have been read
-      if (ok && elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint64_t at = (uint64_t)((kk / 4 * C::BLOCK + kk % 4 * 32) >> 4);
-          mma_smem(tmem + i % NS * kRows, d_q + at, d_k + (uint64_t)((s * C::TILE) >> 4) + at, idesc_s, kk > 0);
-        }
-        commit(k_empty + 8 * s);
-        commit(s_full + 8 * (i % NS));
-      }
-      __syncwarp();
-    };
-    wait(q_full, 0);
-    for (int i = 0; i < AHEAD && i < tiles.count && ok; ++i) scores(i);
-    for (int i = 0; i < tiles.count && ok; ++i) {
-      if (i + AHEAD < tiles.count) scores(i + AHEAD);
-      if (!ok) break;
-      const int s = i % S, k0 = tiles.key(i);
-      wait(v_full + 8 * s, (i / S) & 1);
-      if (ok && k0 + kRows > n) {
-        // values behind the sequence are not zero times a weight of zero where they are no numbers: they go
-        const int gone = k0 + kRows - n;
-        for (int p = lane; p < C::BLOCKS * gone * 8; p += 32) {
-          const int c = p / (gone * 8), r = kRows - gone + p % (gone * 8) / 8;
-          *(uint4*)(vs + s * C::TILE + c * C::BLOCK + r * 128 + p % 8 * 16) = make_uint4(0, 0, 0, 0);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-      }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        wait(p_full + 16 * (i % NS) + 8 * half, (i / NS) & 1);
+    int it = 0, done = 0;
+    for (int unit = blockIdx.x; unit < a.units && ok; unit += gridDim.x) {
+      const Unit<ITEMS> w(a, unit);
+      if (!w.count) continue;
+      auto scores = [&](int u, int i) {
+        const int j = it + i, s = j % S;
+        if (u == 0) wait(K_FULL + s, (j / S) & 1);
         if (ok && elect_one()) {
 #pragma unroll
-          for (int kk = half * (kRows / 32); kk < (half + 1) * (kRows / 32); ++kk)
-            mma_tmem(t_out, tmem + i % NS * kRows + kk * 8, d_v + (uint64_t)((s * C::TILE + kk * 2048) >> 4), idesc_o, i > 0 || kk > 0);
-          if (half) {
-            commit(v_empty + 8 * s);
-            commit(pv_done);
+          for (int kk = 0; kk < DP / 16; ++kk) {
+            const uint64_t at = (uint64_t)((kk / 4 * C::BLOCK + kk % 4 * 32) >> 4);
+            mma_smem(tmem + place(u, j) * kRows, d_q + (uint64_t)((u * C::TILE) >> 4) + at, d_k + (uint64_t)((s * C::TILE) >> 4) + at, idesc_s, kk > 0);
+          }
+          commit(bar(S_FULL + place(u, j)));
+          if (u == ITEMS - 1) {
+            commit(bar(K_EMPTY + s));
+            if (i + 1 == w.count) commit(bar(Q_EMPTY));
           }
         }
         __syncwarp();
+      };
+      auto weighted = [&](int u, int i) {
+        const int j = it + i, s = j % S, k0 = w.key(i);
+        if (u == 0) {
+          wait(V_FULL + s, (j / S) & 1);
+          if (ok && k0 + kRows > w.n) {
+            // values behind the sequence are not zero times a weight of zero where they are no numbers: they go
+            const int gone = k0 + kRows - w.n;
+            for (int p = lane; p < C::BLOCKS * gone * 8; p += 32) {
+              const int c = p / (gone * 8), r = kRows - gone + p % (gone * 8) / 8;
+              *(uint4*)(vs + s * C::TILE + c * C::BLOCK + r * 128 + p % 8 * 16) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+        }
+        if (i == 0 && done) wait(O_EMPTY + u, (done - 1) & 1);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          wait(P_FULL + 2 * place(u, j) + half, turn(j));
+          if (ok && elect_one()) {
+#pragma unroll
+            for (int kk = half * (kRows / 32); kk < (half + 1) * (kRows / 32); ++kk)
+              mma_tmem(outputs(u), tmem + place(u, j) * kRows + C::weights(half) + kk % 4 * 8, d_v + (uint64_t)((s * C::TILE + kk * 2048) >> 4), idesc_o, i > 0 || kk > 0);
+            if (half) {
+              commit(bar(PV_DONE + u));
+              if (u == ITEMS - 1) commit(bar(V_EMPTY + s));
+            }
+          }
+          __syncwarp();
+        }
+      };
+      wait(Q_FULL, done & 1);
+#pragma unroll
+      for (int u = 0; u < ITEMS; ++u) scores(u, 0);
+      for (int i = 0; i < w.count && ok; ++i) {
+        if (ITEMS == 1 && i + 1 < w.count) scores(0, i + 1);
+#pragma unroll
+        for (int u = 0; u < ITEMS; ++u) {
+          weighted(u, i);
+          if (ITEMS == 2 && i + 1 < w.count) scores(u, i + 1);
+        }
       }
+      it += w.count;
+      ++done;
     }
     if (!ok || *failed) {                                            // tensor memory goes back only when no product is left
-      if (elect_one()) commit(drained);
+      if (elect_one()) commit(bar(DRAINED));
       __syncwarp();
-      mbar_wait(drained, 0);
+      mbar_wait(bar(DRAINED), 0);
     }
   } else {
     // ------------------------------ rows: weights, then the result ------------------------------------------------
-    const uint32_t mine = (uint32_t)(32 * warp) << 16;
-    const int row = q0 + tid;
+    constexpr int COLS = C::COLS;
+    const int quad = warp & 3, upper = warp >> 2, u = ITEMS == 2 ? upper : 0, half = ITEMS == 2 ? 0 : upper, r = quad * 32 + lane;
+    const uint32_t mine = (uint32_t)(32 * quad) << 16;
     // f16: weights in units that keep the small ones out of its subnormal range
     constexpr float shift = std::is_same<T, __half>::value ? 6.f : 0.f;
-    float m = neg_inf(), l = 0.f;
+    const uint64_t scale = two(a.scale, a.scale);
     bool ok = true;
-    auto wait = [&](uint32_t bar, int parity) {
-      ok = __all_sync(0xFFFFFFFFu, role_wait(bar, parity, failed));
-      after_sync();
-      return ok;
+    auto wait = [&](int k, int parity) { return ok = __all_sync(0xFFFFFFFFu, role_wait(bar(k), parity, failed)); };
+    int it = 0, spoken = 0;
+    // what the other thread of the row says for what this one says
+    auto exchange = [&](float v, float& other) {
+      float* at = said + (spoken & 1) * 2 * kRows;
+      at[half * kRows + r] = v;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(AGREED + quad));
+      if (!wait(AGREED + quad, spoken & 1)) return false;
+      ++spoken;
+      other = at[(half ^ 1) * kRows + r];
+      return true;
     };
-    for (int i = 0; i < tiles.count; ++i) {
-      const int k0 = tiles.key(i);
-      const uint32_t t_s = tmem + mine + i % NS * kRows;
-      if (!wait(s_full + 8 * (i % NS), (i / NS) & 1)) break;
-      uint32_t s[kRows];
+    for (int unit = blockIdx.x; unit < a.units && ok; unit += gridDim.x) {
+      const Unit<ITEMS> w(a, unit);
+      const int q0 = w.q0[u], row = q0 + r;
+      T* out = (T*)a.out + (((long long)w.b * a.tokens + q0 + quad * 32) * a.heads + w.head[u]) * D;
+      float m = neg_inf(), l = 0.f;
+      for (int i = 0; i < w.count; ++i) {
+        const int j = it + i, k0 = w.key(i) + half * COLS;
+        const uint32_t t_s = tmem + mine + place(u, j) * kRows;
+        if (!wait(S_FULL + place(u, j), turn(j))) break;
+        after_sync();
+        // The scores are read twice, 32 at a time and the next while these are worked on: once for the maximum, once for the weights. (Held
+        // from one to the other, a row's did not stay in registers.)
+        constexpr int PARTS = COLS / 32;
+        uint32_t held[2][32];
+        // masks at the edges only: the last key that the row sees, the first of its window, the sinks
+        const bool late = k0 + COLS - 1 > q0, early = a.window > 0 && q0 + kRows - 1 - k0 >= a.window && k0 + COLS > a.sinks;
+        // (compares and selects run at half the rate of additions: each case has no more of them than it needs, and what they leave goes
+        // back to where the weights' pass reads it)
+        auto masked = [&](uint32_t* s, int c) {
+          const int most = row - k0 - c, least = row - a.window + 1 - k0 - c, always = a.sinks - k0 - c;
+          if (early && always > 0) {
 #pragma unroll
-      for (int c = 0; c < kRows; c += 32) load32(t_s + c, s + c);
-      loaded();
+            for (int k = 0; k < 32; ++k)
+              if (k < least && k >= always) s[k] = 0xFF800000u;
+          } else if (early) {
 #pragma unroll
-      for (int c = 0; c < kRows; c += 32) settle(s + c);
-      // masks at the edges only: the last key that the row sees, the first of its window, the sinks
-      const bool late = k0 + kRows - 1 > q0, early = a.window > 0 && q0 + kRows - 1 - k0 >= a.window && k0 + kRows > a.sinks;
-      if (early && k0 < a.sinks) {
-        const int least = row - a.window + 1 - k0, always = a.sinks - k0;
+            for (int k = 0; k < 32; ++k)
+              if (k < least) s[k] = 0xFF800000u;
+          }
+          if (late) {
 #pragma unroll
-        for (int k = 0; k < kRows; ++k)
-          if (k < least && k >= always) s[k] = 0xFF800000u;
-      } else if (early) {
-        const int least = row - a.window + 1 - k0;
+            for (int k = 0; k < 32; ++k)
+              if (k > most) s[k] = 0xFF800000u;
+          }
+        };
+        float top[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+        load32(t_s + half * COLS, held[0]);
 #pragma unroll
-        for (int k = 0; k < kRows; ++k)
-          if (k < least) s[k] = 0xFF800000u;
-      }
-      if (late) {
-        const int most = row - k0;
+        for (int c = 0; c < PARTS; ++c) {
+          uint32_t* s = held[c & 1];
+          loaded();
+          settle(s);
+          if (c + 1 < PARTS) load32(t_s + half * COLS + (c + 1) * 32, held[(c + 1) & 1]);
+          else if (!(late || early)) load32(t_s + half * COLS, held[0]);                    // the first once more, for the weights
+          if (late || early) {
+            masked(s, c * 32);
+            store32(t_s + half * COLS + c * 32, s);
+          }
 #pragma unroll
-        for (int k = 0; k < kRows; ++k)
-          if (k > most) s[k] = 0xFF800000u;
-      }
-      float top[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
-#pragma unroll
-      for (int k = 0; k < kRows; k += 2) top[k / 2 % 4] = max3(top[k / 2 % 4], __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
-      const float best = fmaxf(max3(top[0], top[1], top[2]), top[3]);
-      const bool grown = best > m && (best - m) * a.scale > kGrowth;
-      if (__any_sync(0xFFFFFFFFu, grown)) {
-        const float now = fmaxf(m, best), keep = m == neg_inf() ? 0.f : power((m - now) * a.scale);
-        m = now;
-        l *= keep;
-        if (i > 0) {
-          if (!wait(pv_done, (i - 1) & 1)) break;
+          for (int k = 0; k < 32; k += 2) top[k / 2 % 4] = max3(top[k / 2 % 4], __uint_as_float(s[k]), __uint_as_float(s[k + 1]));
+        }
+        if (late || early) {
+          stored();
+          load32(t_s + half * COLS, held[0]);
+        }
+        float best = fmaxf(max3(top[0], top[1], top[2]), top[3]);
+        if (ITEMS == 1) {
+          float other;
+          if (!exchange(best, other)) break;
+          best = fmaxf(best, other);
+        }
+        const bool grown = best > m && (best - m) * a.scale > kGrowth;
+        if (__any_sync(0xFFFFFFFFu, grown)) {                          // (of the same rows, so the same in both warps of a row)
+          const float now = fmaxf(m, best), keep = m == neg_inf() ? 0.f : power((m - now) * a.scale);
+          m = now;
+          l *= keep;
+          if (i > 0) {
+            if (!wait(PV_DONE + u, (j - 1) & 1)) break;
+            after_sync();
 #pragma unroll 1
-          for (int c = 0; c < DP; c += 32) {
-            uint32_t o[32];
-            load32(t_out + mine + c, o);
-            loaded();
-            settle(o);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-            store32(t_out + mine + c, o);
+            for (int c = half * (DP / 2); c < (ITEMS == 2 ? DP : (half + 1) * (DP / 2)); c += 8) scale8(outputs(u) + mine + c, keep);
           }
         }
-      }
-      const float ref = m == neg_inf() ? 0.f : m * a.scale - shift;
-      const uint64_t scale = two(a.scale, a.scale), minus = two(-ref, -ref);
-      uint64_t sum[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
+        const float ref = m == neg_inf() ? 0.f : m * a.scale - shift;
+        const uint64_t minus = two(-ref, -ref);
+        uint64_t sum[4] = {0, 0, 0, 0};
         uint32_t p[32];
 #pragma unroll
-        for (int k = 0; k < kRows / 2; k += 2) {
-          const uint64_t x = fma2(two(s[half * (kRows / 2) + k], s[half * (kRows / 2) + k + 1]), scale, minus);
-          const float a0 = power(first(x)), a1 = power(second(x));
-          sum[k / 2 % 4] = add2(sum[k / 2 % 4], two(a0, a1));
-          p[k / 2] = pair16<T>(a0, a1);
-        }
-        store32(t_s + half * 32, p);
-        stored();
-        before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + 16 * (i % NS) + 8 * half);
-      }
-      const uint64_t all = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
-      l += first(all) + second(all);
-    }
-    if (ok && wait(pv_done, (tiles.count - 1) & 1)) {
-      const bool some = row < n;
-      const float inv = some && (l > 0.f || l != l) ? 1.f / l : 0.f;
+        for (int c = 0; c < PARTS; ++c) {
+          uint32_t* s = held[c & 1];
+          loaded();
+          settle(s);
+          if (c + 1 < PARTS) load32(t_s + half * COLS + (c + 1) * 32, held[(c + 1) & 1]);
 #pragma unroll
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t o[32];
-        load32(t_out + mine + c, o);
-        loaded();
-        settle(o);
+          for (int g = 0; g < 32; g += 16) {                            // eight pairs side by side: one after another they are a chain
+            uint64_t x[8];
+            float y[16];
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          if (row < a.tokens && c + e < D) {
-            uint4 v = {0, 0, 0, 0};
-            if (some) {
-              v.x = pair16<T>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-              v.y = pair16<T>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-              v.z = pair16<T>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-              v.w = pair16<T>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-            }
-            *(uint4*)(out + tid * pitch + c + e) = v;
+            for (int k = 0; k < 8; ++k) x[k] = fma2(two(s[g + 2 * k], s[g + 2 * k + 1]), scale, minus);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) { y[2 * k] = power(first(x[k])); y[2 * k + 1] = power(second(x[k])); }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum[k % 4] = add2(sum[k % 4], two(y[2 * k], y[2 * k + 1]));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) p[c % 2 * 16 + g / 2 + k] = pair16<T>(y[2 * k], y[2 * k + 1]);
+          }
+          if (c % 2 == 1) {
+            // the weights of 64 keys take the place of scores that this thread has read
+            const int part = ITEMS == 2 ? c / 2 : half;
+            store32(t_s + C::weights(part), p);
+            stored();
+            before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(P_FULL + 2 * place(u, j) + part));
           }
         }
+        const uint64_t all = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+        l += first(all) + second(all);
+      }
+      if (!ok) break;
+      if (w.count) {
+        if (ITEMS == 1) {
+          float other;
+          if (!exchange(l, other)) break;
+          l += other;
+        }
+        it += w.count;
+        if (!wait(PV_DONE + u, (it - 1) & 1)) break;
+        after_sync();
+      }
+      const bool some = w.count && row < w.n;
+      const float inv = some && (l > 0.f || l != l) ? 1.f / l : 0.f;
+#pragma unroll
+      for (int c0 = 0; c0 < (ITEMS == 2 ? DP : DP / 2); c0 += 32) {
+        const int c = (ITEMS == 2 ? 0 : half * (DP / 2)) + c0;
+        uint32_t o[32];
+        if (w.count) {
+          load32(outputs(u) + mine + c, o);
+          loaded();
+          settle(o);
+        }
+        // by way of shared memory, so that a store touches eight rows' 64 bytes and not 32 rows' 16: those took @8600@ cycles a tile
+        uint8_t* at = stage + warp * 32 * kStagePitch;
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          uint4 v = {0, 0, 0, 0};
+          if (some) {
+            v.x = pair16<T>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+            v.y = pair16<T>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+            v.z = pair16<T>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+            v.w = pair16<T>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+          }
+          *(uint4*)(at + lane * kStagePitch + e * 2) = v;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int line = e * 8 + lane / 4, col = c + lane % 4 * 8;
+          if (q0 + quad * 32 + line < a.tokens && col < D) *(uint4*)(out + (long long)line * a.heads * D + col) = *(const uint4*)(at + line * kStagePitch + lane % 4 * 16);
+        }
+        __syncwarp();
+      }
+      if (w.count) {
+        before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(O_EMPTY + u));
       }
     }
   }
   before_sync();
   __syncthreads();
   if (tid == 0 && *failed) atomicAdd(error_flag, 1);
-  if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLUMNS) : "memory");
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 size_t fma_smem(int dim) { return (size_t)(3 * kTile * (dim + 4) + kTile * kScoreRow) * 4; }
@@ -533,10 +682,11 @@ cudaError_t launch_fma(const Prompt& a, cudaStream_t stream, int* launches) {
                    stream, launches, a);
 }
 
-template <typename T, int DP>
-cudaError_t launch_mma(const Prompt& a, int* error_flag, cudaStream_t stream, int* launches, const char** why) {
+template <typename T, int DP, int ITEMS>
+cudaError_t launch_mma(Prompt a, int* error_flag, cudaStream_t stream, int* launches, const char** why) {
   static bool done[64] = {};
-  if (cudaError_t e = allow_smem(prompt_mma_kernel<T, DP>, Mma<DP>::SMEM, done)) return e;
+  using C = Mma<DP, ITEMS>;
+  if (cudaError_t e = allow_smem(prompt_mma_kernel<T, DP, ITEMS>, C::SMEM, done)) return e;
   // features, tokens of all sequences, heads: boxes of 64 features and 128 tokens of one head; what is outside reads zero
   alignas(64) CUtensorMap maps[3];
   const void* bases[3] = {a.q, a.k, a.v};
@@ -549,14 +699,21 @@ cudaError_t launch_mma(const Prompt& a, int* error_flag, cudaStream_t stream, in
       return cudaErrorInvalidValue;
     }
   }
-  return launch_op(prompt_mma_kernel<T, DP>, dim3((unsigned)a.heads, (unsigned)((a.tokens + kRows - 1) / kRows), (unsigned)a.batch), kMmaThreads, Mma<DP>::SMEM, stream,
-                   launches, maps[0], maps[1], maps[2], a, error_flag);
+  const int tiles = (a.tokens + kRows - 1) / kRows;
+  a.pairs = ITEMS == 2 && a.group % 2 == 0;
+  a.head_units = a.pairs ? a.heads / 2 : a.heads;
+  a.query_units = ITEMS == 2 && !a.pairs ? (tiles + 1) / 2 : tiles;
+  a.units = a.head_units * a.query_units * a.batch;
+  return launch_op(prompt_mma_kernel<T, DP, ITEMS>, dim3((unsigned)std::min(a.units, kSMs)), kMmaThreads, C::SMEM, stream, launches, maps[0], maps[1], maps[2], a,
+                   error_flag);
 }
 template <typename T>
 cudaError_t launch_16bit(const Prompt& a, int* error_flag, cudaStream_t stream, int* launches, const char** why) {
-  if (a.dim <= 64) return launch_mma<T, 64>(a, error_flag, stream, launches, why);
-  if (a.dim <= 128) return launch_mma<T, 128>(a, error_flag, stream, launches, why);
-  return launch_mma<T, 256>(a, error_flag, stream, launches, why);
+  // two tiles of queries a block where that still leaves no SM without one
+  const bool two = (long long)a.heads * a.batch * ((a.tokens + kRows - 1) / kRows) >= 2 * kSMs;
+  if (a.dim <= 64) return two ? launch_mma<T, 64, 2>(a, error_flag, stream, launches, why) : launch_mma<T, 64, 1>(a, error_flag, stream, launches, why);
+  if (a.dim <= 128) return two ? launch_mma<T, 128, 2>(a, error_flag, stream, launches, why) : launch_mma<T, 128, 1>(a, error_flag, stream, launches, why);
+  return launch_mma<T, 256, 1>(a, error_flag, stream, launches, why);
 }
 
 }  // namespace
@@ -565,6 +722,7 @@ const char* window_attention_plan(OperatorLaunch& op) {
   if (op.heads > 65535 || op.batch > 65535) return "more than 65535 heads or sequences";
   if (op.tokens > 65535 * kTile) return "prompts of more than 65535 tiles of 64 tokens";
   if ((long long)op.batch * op.tokens >= (1LL << 31)) return "2^31 tokens and more";
+  if ((long long)op.batch * op.heads * ((op.tokens + kRows - 1) / kRows) >= (1LL << 31) - kSMs) return "too many heads and sequences";
   op.scratch_bytes = 0;
   op.launches = 1;
   op.waits = op.type != 0;
