@@ -1282,6 +1282,66 @@ struct DecodeAttentionFusion {
   }
 };
 
+// A loss and its gradient: b200.token_log_probs and the b200.token_log_probs_grad of the same logits become one operation that reads the
+// logits once, where the rows fit (token_log_probs_at_once) and the cotangents do not depend on the log probabilities. What the
+// cotangents are made of moves in front of it.
+// ---------------------------------------------------------------------------
+void join_loss_and_gradient(Block* b) {
+  for (auto& op : b->ops)
+    for (auto& r : op->regions) join_loss_and_gradient(r.get());
+  for (size_t g = 0; g < b->ops.size(); g++) {
+    Op* grad = b->ops[g].get();
+    if (grad->name != "b200.token_log_probs_grad" || grad->operands.size() != 8 || grad->results.size() != 1) continue;
+    Op* probs = grad->operands[2]->def;
+    if (!probs || probs->parent != b || probs->name != "b200.token_log_probs" || probs->results.size() != 4 || probs->operands.size() != 2) continue;
+    if (grad->operands[0] != probs->operands[0] || grad->operands[1] != probs->operands[1] || grad->operands[2] != probs->results[2] ||
+        grad->operands[3] != probs->results[3] || grad->operands[4] != probs->results[1])
+      continue;
+    const TensorType& x = probs->operands[0]->type;
+    if (x.rank() != 2 || (x.dt != DT::F32 && x.dt != DT::BF16 && x.dt != DT::F16) || x.dims[1] >= (1LL << 30)) continue;
+    OperatorLaunch o;
+    o.type = x.dt == DT::F32 ? 0 : 1;
+    o.rows = x.dims[0];
+    o.vocab = (int)x.dims[1];
+    if (!token_log_probs_at_once(o)) continue;
+    // the operations of this block that the cotangents need
+    std::set<Op*> need;
+    std::function<bool(Value*)> collect = [&](Value* v) {
+      Op* d = v->def;
+      if (!d || d->parent != b || need.count(d)) return true;
+      if (d == probs || d == grad || !d->regions.empty()) return false;
+      need.insert(d);
+      for (Value* in : d->operands)
+        if (!collect(in)) return false;
+      return true;
+    };
+    bool free = true;
+    for (int k = 5; k < 8; k++) free = free && collect(grad->operands[k]);
+    if (!free) continue;
+    std::vector<std::unique_ptr<Op>> before, after;
+    std::unique_ptr<Op> joined;
+    bool past = false;
+    for (auto& up : b->ops) {
+      if (up.get() == probs) { joined = std::move(up); past = true; continue; }
+      if (up.get() == grad) continue;
+      (past && !need.count(up.get()) ? after : before).push_back(std::move(up));
+    }
+    joined->name = "b200.token_log_probs_both";
+    for (int k = 5; k < 8; k++) joined->operands.push_back(grad->operands[k]);
+    Value* dx = grad->results[0];
+    dx->def = joined.get();
+    dx->def_index = 4;
+    joined->results.push_back(dx);
+    std::unique_ptr<Op> gone;
+    for (auto& up : b->ops)
+      if (up && up.get() == grad) gone = std::move(up);
+    before.push_back(std::move(joined));
+    for (auto& up : after) before.push_back(std::move(up));
+    b->ops = std::move(before);
+    g = (size_t)-1;                                          // positions changed: start over
+  }
+}
+
 // ---------------------------------------------------------------------------
 // op classification
 // ---------------------------------------------------------------------------
@@ -1291,7 +1351,7 @@ Cat categorize(Op* op) {
   const std::string sh = op->short_name();
   if (sh == "return") return Cat::RETURN;
   if (op->name == "b200.decode_attention") return Cat::ATTENTION;
-  if (is_operator(op->name)) return Cat::OPERATOR;
+  if (is_operator(op->name) || op->name == "b200.token_log_probs_both") return Cat::OPERATOR;
   if (op->name.rfind("stablehlo.", 0) != 0 && op->name.rfind("chlo.", 0) != 0 && op->name.rfind("mhlo.", 0) != 0)
     return Cat::UNSUPPORTED;
   if (is_elementwise_op(sh)) return Cat::ELEMENTWISE;
@@ -2963,10 +3023,10 @@ struct Planner {
       if (o.has_lengths) want(in[3], "the lengths", DT::I32, {qd[0]});
       want(out[0], "the result", q->type.dt, qd);
     } else {
-      const bool grad = op->name == "b200.token_log_probs_grad";
-      o.kind = grad ? OperatorLaunch::TOKEN_LOG_PROBS_GRAD : OperatorLaunch::TOKEN_LOG_PROBS;
+      const bool grad = op->name == "b200.token_log_probs_grad", both = op->name == "b200.token_log_probs_both";
+      o.kind = grad ? OperatorLaunch::TOKEN_LOG_PROBS_GRAD : both ? OperatorLaunch::TOKEN_LOG_PROBS_BOTH : OperatorLaunch::TOKEN_LOG_PROBS;
       o.top = grad ? 0 : (int)whole("top", 0, 0, 128);
-      count(grad ? 8 : 2, grad ? 8 : 2, grad ? 1 : o.top ? 6 : 4);
+      if (!both) count(grad ? 8 : 2, grad ? 8 : 2, grad ? 1 : o.top ? 6 : 4);
       o.type = type_of(in[0], "the logits");
       rank(in[0], "the logits", 2);
       o.rows = in[0]->type.dims[0];
@@ -2974,7 +3034,9 @@ struct Planner {
       if (o.vocab < 1) fail("the vocabulary is empty");
       if (o.top > o.vocab) fail("more alternatives (" + std::to_string(o.top) + ") than the vocabulary has (" + std::to_string(o.vocab) + ")");
       want(in[1], "the tokens", DT::I32, {o.rows});
-      if (grad) {
+      if (both) {
+        for (int k = 2; k < 5; k++) want(in[k], "a cotangent", DT::F32, {o.rows});
+      } else if (grad) {
         for (int k = 2; k < 8; k++) want(in[k], "an operand of the gradient", DT::F32, {o.rows});
         want(out[0], "the result", in[0]->type.dt, in[0]->type.dims);
       } else {
@@ -6877,6 +6939,7 @@ std::unique_ptr<CompiledProgram> compile_module(Module& m, const CompileOptions&
     split_counted_loops(m, f->body.get(), Planner::loop_product_model(opts.tensor_cores));
   SkinnyWeightHoist(m).run(f->body.get());
   DecodeAttentionFusion(m).run(f->body.get());
+  if (opts.fuse) join_loss_and_gradient(f->body.get());
   // unsupported-op check names every offender at once (src/pjrt_plugin/stablehlo_parser.cc:167-184)
   std::set<std::string> bad;
   collect_unsupported(f->body.get(), bad, false);

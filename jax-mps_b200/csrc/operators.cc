@@ -12,6 +12,7 @@ const char* operator_name(const OperatorLaunch& op) {
     case OperatorLaunch::WINDOW_ATTENTION: return "b200.window_attention";
     case OperatorLaunch::TOKEN_LOG_PROBS: return "b200.token_log_probs";
     case OperatorLaunch::TOKEN_LOG_PROBS_GRAD: return "b200.token_log_probs_grad";
+    case OperatorLaunch::TOKEN_LOG_PROBS_BOTH: return "b200.token_log_probs_both";
     default: return "none";
   }
 }
@@ -20,7 +21,7 @@ const char* operator_plan(OperatorLaunch& op) {
   switch (op.kind) {
     case OperatorLaunch::PAGED_ATTENTION: return paged_attention_plan(op);
     case OperatorLaunch::WINDOW_ATTENTION: return window_attention_plan(op);
-    case OperatorLaunch::TOKEN_LOG_PROBS: case OperatorLaunch::TOKEN_LOG_PROBS_GRAD: return token_log_probs_plan(op);
+    case OperatorLaunch::TOKEN_LOG_PROBS: case OperatorLaunch::TOKEN_LOG_PROBS_GRAD: case OperatorLaunch::TOKEN_LOG_PROBS_BOTH: return token_log_probs_plan(op);
     default: return "no operator";
   }
 }
@@ -30,6 +31,7 @@ cudaError_t launch_operator(const OperatorLaunch& op, void* const* args, void* s
     case OperatorLaunch::PAGED_ATTENTION: return launch_paged_attention(op, args, scratch, stream, launches);
     case OperatorLaunch::WINDOW_ATTENTION: return launch_window_attention(op, args, scratch, error_flag, stream, launches, why);
     case OperatorLaunch::TOKEN_LOG_PROBS: return launch_token_log_probs(op, args, scratch, stream, launches);
+    case OperatorLaunch::TOKEN_LOG_PROBS_BOTH: return launch_token_log_probs_both(op, args, stream, launches);
     case OperatorLaunch::TOKEN_LOG_PROBS_GRAD: return launch_token_log_probs_grad(op, args, stream, launches);
     default: return cudaErrorInvalidValue;
   }

@@ -7,7 +7,7 @@
 namespace b200 {
 
 struct OperatorLaunch {
-  enum Kind { NONE, PAGED_ATTENTION, WINDOW_ATTENTION, TOKEN_LOG_PROBS, TOKEN_LOG_PROBS_GRAD } kind = NONE;
+  enum Kind { NONE, PAGED_ATTENTION, WINDOW_ATTENTION, TOKEN_LOG_PROBS, TOKEN_LOG_PROBS_GRAD, TOKEN_LOG_PROBS_BOTH } kind = NONE;
   int type = 0;                             // of the data: 0 f32, 1 bf16, 2 f16
   // attention: sequences, tokens of each (prompt), query and key-value heads, features of a head
   int batch = 0, tokens = 0, heads = 0, kv_heads = 0, dim = 0;
@@ -39,6 +39,9 @@ const char* window_attention_plan(OperatorLaunch& op);
 cudaError_t launch_window_attention(const OperatorLaunch& op, void* const* args, void* scratch, int* error_flag, cudaStream_t stream, int* launches, const char** why);
 const char* token_log_probs_plan(OperatorLaunch& op);
 cudaError_t launch_token_log_probs(const OperatorLaunch& op, void* const* args, void* scratch, cudaStream_t stream, int* launches);
+// Log probabilities and their gradient by one reading of the logits: results, gradient, logits, tokens, the three cotangents.
+bool token_log_probs_at_once(const OperatorLaunch& op);
+cudaError_t launch_token_log_probs_both(const OperatorLaunch& op, void* const* args, cudaStream_t stream, int* launches);
 cudaError_t launch_token_log_probs_grad(const OperatorLaunch& op, void* const* args, cudaStream_t stream, int* launches);
 
 // Moves inside a cache. `token`: bytes of one token's keys (or values) of one layer; planes = layers * 2. The index arrays are

@@ -3053,6 +3053,7 @@ b200_error* cache_shape(b200_client* c, const b200_buffer* cache, CacheShape* sh
   if (shape->planes > 65535) return make_error(B200_INVALID_ARGUMENT, "a cache of more than 32767 layers");
   if (shape->pages > INT32_MAX || shape->page > INT32_MAX || shape->pages * shape->page > INT32_MAX)
     return make_error(B200_INVALID_ARGUMENT, "a cache of 2^31 positions and more");
+  if (shape->page * shape->token > (1LL << 34)) return make_error(B200_INVALID_ARGUMENT, "a page of more than 16 GB");
   return nullptr;
 }
 

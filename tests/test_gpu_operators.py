@@ -316,6 +316,28 @@ def test_gradient_of_token_log_probs(client, dt, R, V):
     check_probs(client, x, tokens, 0, dt, g)
 
 
+@pytest.mark.parametrize("dt,R,V", [("f32", 299, 4097), ("f32", 300, 8190), ("f32", 296, 32760), ("f32", 296, 32761), ("bf16", 297, 20001), ("f16", 450, 8192)])
+def test_loss_and_gradient_by_one_reading(client, dt, R, V):
+    rng = np.random.default_rng(V)
+    x = rounded(rng.standard_normal((R, V)) * 3, dt)
+    x[5, ::3] = -np.inf
+    x[6] = -np.inf
+    x[6, V - 1] = 1.0
+    x[7] = np.float32(-3e38) if dt == "f32" else x[7]
+    tokens = rng.integers(0, V, R)
+    tokens[::4], tokens[5], tokens[6] = -100, 1, V - 1
+    g = [rng.standard_normal(R).astype(np.float32) for _ in range(3)]
+    # (a row of the lowest value has no span: its probabilities are even, and tested as such)
+    keep = np.arange(R) != 7
+    got = run(client, lambda b, x, t, *g: (lambda o: o + b.grad(b.reduce_sum(b.add(b.add(b.mul(o[0], g[0]), b.mul(o[1], g[1])), b.mul(o[2], g[2])), (0,)), [x]))(
+        b.token_log_probs(x, t)), [x, tokens.astype(np.int32), *g], [dt, "i32", "f32", "f32", "f32"])
+    if dt == "f32":
+        np.testing.assert_allclose(got[1][7], np.log(V), rtol=1e-6)
+        p7 = g[2][7] - (g[0][7] if tokens[7] >= 0 else 0.0)
+        np.testing.assert_allclose(np.delete(got[3][7], max(tokens[7], 0)), p7 / V, rtol=1e-4, atol=abs(g[1][7]) * 1e-5 / V + 1e-30)
+    check_probs(client, x[keep], tokens[keep], 0, dt, [c[keep] for c in g])
+
+
 def test_gradient_where_the_vocabulary_is_masked(client):
     rng = np.random.default_rng(6)
     x = (rng.standard_normal((4, 999)) * 2).astype(np.float32)

@@ -33,6 +33,32 @@ def test_programs_with_operators_compile(dt):
     assert "operator token_log_probs " in plan and "operator token_log_probs_grad" in plan
 
 
+def loss_text(R, V, dt, dependent=False, top=0):
+    b = Builder()
+    x, t, w = b.arg((R, V), dt), b.arg((R,), "i32"), b.arg((R,), "f32")
+    lp, h, n, *best = b.token_log_probs(x, t, top=top)
+    # the weights of the log probabilities, scaled behind them in the program; or the entropies, which the call itself gives
+    scaled = h if dependent else b.mul(w, b.full((R,), 0.5, "f32"))
+    dx = b.grad(b.reduce_sum(b.mul(lp, scaled), (0,)), [x])[0]
+    return b.module([b.reduce_sum(b.mul(lp, w), (0,)), dx, n, *best])
+
+
+def test_loss_and_gradient_become_one_operation():
+    def operators_in(*a, **kw):
+        plan, _ = b200.compile_to_plan(loss_text(*a, **kw))
+        return [w for w in plan.split() if w.startswith("token_log_probs")]
+    assert operators_in(300, 5000, "f32") == ["token_log_probs_both"]
+    assert operators_in(296, 32760, "f32") == ["token_log_probs_both"] and operators_in(296, 65520, "bf16") == ["token_log_probs_both"]
+    two = ["token_log_probs", "token_log_probs_grad"]
+    assert operators_in(295, 5000, "f32") == two and operators_in(296, 32761, "f32") == two and operators_in(300, 500, "f32") == two
+    assert operators_in(300, 5000, "f32", dependent=True) == two and operators_in(300, 5000, "f32", top=3) == two
+    text = loss_text(300, 4100, "f32")
+    rng = np.random.default_rng(0)
+    args = [rng.standard_normal((300, 4100)).astype(np.float32), rng.integers(-1, 4100, 300).astype(np.int32), rng.standard_normal(300).astype(np.float32)]
+    got = interp.run_text(text, args, wide=True)
+    np.testing.assert_allclose(got[1], operators.token_log_probs_grad(args[0], args[1], args[2] * 0.5, np.zeros(300), np.zeros(300)), rtol=1e-5, atol=1e-9)
+
+
 def test_the_assembly_jax_prints():
     # jax.ffi.ffi_call(...)(q, ...): the dictionary stands under one of two names
     for attr in ("backend_config = {layer = 1 : i64, window = 5 : i64}, api_version = 4 : i32", "mhlo.backend_config = {layer = 1 : i64, window = 5 : i64}"):
