@@ -635,6 +635,109 @@ def lstm_inputs(prog: Program, seed: int = 0) -> list:
     return out
 
 
+def _gemma_layer(b: Builder, W: dict, p: str, ops, x: Val, cos: Val, sin: Val, heads: int, head_dim: int, dtype: str, attend):
+    """One decoder layer on x f32[rows, dim] with the rotary angles of its rows; `attend(q, k, v)` maps q `dtype`[rows, heads, head_dim] and
+    the rows' own k, v `dtype`[rows, 1, head_dim] to f32[rows, heads * head_dim]. Returns the new x and (k, v)."""
+    rms_norm, rope, gelu, lin = ops
+    rows = x.shape[0]
+    h = rms_norm(b, x, W[p + "attn_norm"])
+    q = b.convert(rope(b, b.reshape(lin(b, h, W[p + "wq"]), (rows, heads, head_dim)), cos, sin), dtype)
+    k = b.convert(rope(b, b.reshape(lin(b, h, W[p + "wk"]), (rows, 1, head_dim)), cos, sin), dtype)
+    v = b.convert(b.reshape(lin(b, h, W[p + "wv"]), (rows, 1, head_dim)), dtype)
+    x = b.add(x, lin(b, attend(q, k, v), W[p + "wo"]))
+    h2 = rms_norm(b, x, W[p + "mlp_norm"])
+    ff = b.mul(gelu(b, lin(b, h2, W[p + "w_gate"])), lin(b, h2, W[p + "w_up"]))
+    return b.add(x, lin(b, ff, W[p + "w_down"])), (k, v)
+
+
+def _gemma_angles(b: Builder, pos: Val, head_dim: int):
+    """Cosines and sines f32[rows, head_dim / 2] of the rotary embedding at positions f32[rows]."""
+    half = head_dim // 2
+    inv_freq = b.const_array((1.0 / (10000.0 ** (np.arange(half, dtype=np.float64) * 2 / head_dim))).astype(np.float32))
+    ang = b.mul(b.bcast(pos, (pos.shape[0], half), (0,)), b.bcast(inv_freq, (pos.shape[0], half), (1,)))
+    return b.cos(ang), b.sin(ang)
+
+
+def _cache_rows(b: Builder, kvs: list) -> Val:
+    """The layers' (k, v) [rows, 1, head_dim] as [layers, 2, rows, 1, head_dim], the form that goes into a cache of pages."""
+    rows, one, hd = kvs[0][0].shape
+    return b.reshape(b.concatenate([b.reshape(t, (1, rows, one, hd)) for kv in kvs for t in kv], 0), (len(kvs), 2, rows, one, hd))
+
+
+def gemma_paged_prefill(vocab: int = 256000, dim: int = 2048, layers: int = 18, heads: int = 8, head_dim: int = 256, hidden: int = 16384,
+                        batch: int = 4, prompt_len: int = 512, window: int = 0, sinks: int = 0, dtype: str = "bf16") -> Program:
+    """The decoder of `gemma_prefill` on a padded batch of prompts for serving from a cache of pages: attention is causal within each prompt, with
+    a sliding window and sinks where `window` is set. Arguments: the weights, prompts i32[batch, prompt_len], their lengths
+    i32[batch] (one at least). Results: the first generated tokens i32[batch], their log probabilities and the entropies f32[batch], and the keys and
+    values `dtype`[layers, 2, batch * prompt_len, 1, head_dim] of all positions, which `PagedCache.write` takes (those behind a prompt's
+    length for the slot -1)."""
+    spec = gemma_param_spec(vocab, dim, layers, heads, head_dim, hidden)
+    B, T = batch, prompt_len
+    b = Builder()
+    W = {n: b.arg(s, dtype) for n, s in spec}
+    prompts, lengths = b.arg((B, T), "i32"), b.arg((B,), "i32")
+    ops = _gemma_ops(dim, heads, head_dim, dtype)
+    cos, sin = _gemma_angles(b, b.reshape(b.bcast(b.convert(b.iota((T,), "i32", 0), "f32"), (B, T), (1,)), (B * T,)), head_dim)
+    x = b.convert(b.take_rows(W["embed"], b.reshape(prompts, (B * T,))), "f32")
+    x = b.mul(x, b.full(x.shape, math.sqrt(dim), "f32"))
+
+    def attend(q, k, v):
+        o = b.window_attention(b.reshape(q, (B, T, heads, head_dim)), b.reshape(k, (B, T, 1, head_dim)), b.reshape(v, (B, T, 1, head_dim)), lengths,
+                               window=window, sinks=sinks)
+        return b.convert(b.reshape(o, (B * T, heads * head_dim)), "f32")
+    kvs = []
+    for i in range(layers):
+        x, kv = _gemma_layer(b, W, f"layer{i}.", ops, x, cos, sin, heads, head_dim, dtype, attend)
+        kvs.append(kv)
+    last = b.add(b.mul(b.iota((B,), "i32", 0), b.full((B,), T, "i32")), b.sub(lengths, b.full((B,), 1, "i32")))
+    tok, lp, ent = _greedy(b, W, ops, b.take_rows(x, last), dtype)
+    text = b.module([tok, lp, ent, _cache_rows(b, kvs)], name="jit_paged_prefill")
+    args = [(n, s, dtype) for n, s in spec] + [("prompts", (B, T), "i32"), ("lengths", (B,), "i32")]
+    res = [("tokens", (B,), "i32"), ("log_probs", (B,), "f32"), ("entropies", (B,), "f32"), ("rows", (layers, 2, B * T, 1, head_dim), dtype)]
+    return Program("gemma_paged_prefill", text, args, res, 1, {"vocab": vocab, "dim": dim, "layers": layers, "batch": B, "prompt_len": T})
+
+
+def gemma_paged_step(vocab: int = 256000, dim: int = 2048, layers: int = 18, heads: int = 8, head_dim: int = 256, hidden: int = 16384,
+                     batch: int = 4, pages: int = 256, page_size: int = 16, width: int = 64, window: int = 0, sinks: int = 0,
+                     dtype: str = "bf16") -> Program:
+    """One greedy decode step of a batch of sequences whose keys and values lie in pages (the decoder of `gemma_decode_loop`): a token per sequence
+    at the position behind its cached ones. Arguments: the weights, tokens i32[batch], the cache `dtype`[layers, 2, pages, page_size, 1,
+    head_dim], the page table i32[batch, width], lengths i32[batch]. Results: the next tokens i32[batch], their log probabilities and the
+    entropies f32[batch], and the step's keys and values `dtype`[layers, 2, batch, 1, head_dim], which `PagedCache.write` puts behind the
+    cached ones."""
+    spec = gemma_param_spec(vocab, dim, layers, heads, head_dim, hidden)
+    B = batch
+    b = Builder()
+    W = {n: b.arg(s, dtype) for n, s in spec}
+    tokens, cache = b.arg((B,), "i32"), b.arg((layers, 2, pages, page_size, 1, head_dim), dtype)
+    table, lengths = b.arg((B, width), "i32"), b.arg((B,), "i32")
+    ops = _gemma_ops(dim, heads, head_dim, dtype)
+    cos, sin = _gemma_angles(b, b.convert(lengths, "f32"), head_dim)
+    x = b.convert(b.take_rows(W["embed"], tokens), "f32")
+    x = b.mul(x, b.full(x.shape, math.sqrt(dim), "f32"))
+    kvs = []
+    for i in range(layers):
+        def attend(q, k, v, i=i):
+            new = b.reshape(b.concatenate([b.reshape(t, (1, B, 1, head_dim)) for t in (k, v)], 0), (2, B, 1, head_dim))
+            o = b.paged_attention(q, cache, table, lengths, new=new, layer=i, window=window, sinks=sinks)
+            return b.convert(b.reshape(o, (B, heads * head_dim)), "f32")
+        x, kv = _gemma_layer(b, W, f"layer{i}.", ops, x, cos, sin, heads, head_dim, dtype, attend)
+        kvs.append(kv)
+    tok, lp, ent = _greedy(b, W, ops, x, dtype)
+    text = b.module([tok, lp, ent, _cache_rows(b, kvs)], name="jit_paged_step")
+    args = [(n, s, dtype) for n, s in spec] + [("tokens", (B,), "i32"), ("cache", cache.shape, dtype), ("table", (B, width), "i32"), ("lengths", (B,), "i32")]
+    res = [("tokens", (B,), "i32"), ("log_probs", (B,), "f32"), ("entropies", (B,), "f32"), ("rows", (layers, 2, B, 1, head_dim), dtype)]
+    return Program("gemma_paged_step", text, args, res, 1, {"vocab": vocab, "dim": dim, "layers": layers, "batch": B, "pages": pages, "page_size": page_size})
+
+
+def _greedy(b: Builder, W: dict, ops, x: Val, dtype: str):
+    """The most probable next tokens of x f32[rows, dim], their log probabilities, the entropies."""
+    hf = b.convert(ops[0](b, x, W["final_norm"]), dtype)
+    logits = b.convert(b.dot_general(hf, W["embed"], ((1,), (1,))), "f32")
+    tok = b.argmax(logits, 1)
+    return tok, *b.token_log_probs(logits, tok)[:2]
+
+
 def decode_attention(G, M, T, D, N, dt="bf16", masked=True, out_f32=True, scale=True, keepdims=False) -> str:
     """Attention of M query rows per group over T cached positions, the chain a decode step contains
     (examples/gemma/model.py:186-230 of the reference): q [G, M, D] (or [M, D] when G is None), k [.., T, D],
