@@ -2939,7 +2939,8 @@ struct Planner {
       const std::string& raw = op->attr(name);
       char* end = nullptr;
       const double v = strtod(raw.c_str(), &end);
-      if (end == raw.c_str() || !std::isfinite(v)) fail(std::string("attribute ") + name + " is no number: " + raw);
+      // (a float in hexadecimal is the bits of one that has no decimal form)
+      if (end == raw.c_str() || !std::isfinite(v) || raw.find_first_of("xX") != std::string::npos) fail(std::string("attribute ") + name + " is no number: " + raw);
       return v;
     };
     auto whole = [&](const char* name, long long otherwise, long long lo, long long hi) {

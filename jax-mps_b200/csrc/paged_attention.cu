@@ -226,6 +226,9 @@ __global__ void __launch_bounds__(Ring<T, DP, NT>::WARPS * 32, Ring<T, DP, NT>::
   using R = Ring<T, DP, NT>;
   constexpr bool WIDE = sizeof(T) == 4;
   constexpr int HEADS = 8 * NT, S = R::STAGES, W = R::WARPS, STEP = WIDE ? 8 : 16, KSTEPS = DP / STEP;
+  // f16: weights, sums and outputs in units of 2^-14, so that weights keep their bits down to 2^-28 of the largest and no long row of
+  // small ones is lost (they end at 2^-24 otherwise, which 60000 positions make 2^-8 of the result)
+  constexpr float LIFT = std::is_same<T, __half>::value ? 14.f : 0.f;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ float stats[W][HEADS][2];
   const int D = a.dim, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row_pieces = D * (int)sizeof(T) / 16;
@@ -377,8 +380,8 @@ __global__ void __launch_bounds__(Ring<T, DP, NT>::WARPS * 32, Ring<T, DP, NT>::
           const float ref = top == neg_inf() ? 0.f : top;
           keep[t][i] = power(m[t][i] - ref);
           m[t][i] = top;
-          p[i] = power(x - ref);
-          p[2 + i] = power(y - ref);
+          p[i] = power(LIFT > 0.f ? x - ref + LIFT : x - ref);
+          p[2 + i] = power(LIFT > 0.f ? y - ref + LIFT : y - ref);
           l[t][i] = l[t][i] * keep[t][i] + p[i] + p[2 + i];
         }
         if (WIDE) {

@@ -292,6 +292,7 @@ struct StatusWord {
 // whose kernels wait for nothing are not watched at all.
 struct ExecStatus {
   std::shared_ptr<StatusWord> before, after;
+  uint64_t first = 0, last = 0;         // numbers of the executions on their client, from the first to the last
   bool failed() const { return before && after && *after->word != *before->word; }
 };
 
@@ -408,6 +409,7 @@ struct b200_client {
   int* status_block = nullptr;          // pinned words handed to executions
   static constexpr int kStatusWords = 8192;
   std::shared_ptr<StatusWord> last_status;      // the counter behind the last watched execution; null: not known
+  uint64_t watched_executions = 0;
   // Small parts that executions and buffers hand back and forth: free status words and events (under a lock of their
   // own, taken by destructors on any thread).
   std::mutex parts_mu;
@@ -2553,6 +2555,7 @@ b200_error* b200_executable_execute(b200_executable* exe, b200_buffer* const* ar
   std::shared_ptr<ExecStatus> status;
   if (exe->lp->watched || c->armed_wait_polls > 0) {
     status = std::make_shared<ExecStatus>();
+    status->first = status->last = ++c->watched_executions;
     status->before = c->last_status;
     status->after = new_status_word(c);
     if (!status->before && (status->before = new_status_word(c)))
@@ -3058,13 +3061,20 @@ b200_error* cache_shape(b200_client* c, const b200_buffer* cache, CacheShape* sh
 }
 
 // Whether one of n indices below `limit`, `stride` apart, comes twice (negative ones aside). A few are compared with one another, many
-// marked in a bit for each that there can be (sorted, 4099 slots took 110 us).
+// marked in a bit for each that there can be (sorted, 4099 slots took 110 us), unless clearing those would take longer than to sort.
 bool repeats(const int32_t* index, size_t n, size_t stride, int64_t limit) {
   if (n <= 32) {
     for (size_t i = 0; i < n; i++)
       for (size_t j = 0; j < i; j++)
         if (index[i * stride] >= 0 && index[i * stride] == index[j * stride]) return true;
     return false;
+  }
+  if ((size_t)limit / 64 > 32 * n) {
+    std::vector<int32_t> sorted;
+    for (size_t k = 0; k < n; k++)
+      if (index[k * stride] >= 0) sorted.push_back(index[k * stride]);
+    std::sort(sorted.begin(), sorted.end());
+    return std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end();
   }
   std::vector<uint64_t> seen((size_t)(limit + 63) / 64, 0);
   for (size_t k = 0; k < n; k++) {
@@ -3075,6 +3085,20 @@ bool repeats(const int32_t* index, size_t n, size_t stride, int64_t limit) {
     seen[v >> 6] |= bit;
   }
   return false;
+}
+
+// What is known of a buffer that two executions wrote: the counter from in front of the first to behind the last.
+std::shared_ptr<ExecStatus> both_statuses(const std::shared_ptr<ExecStatus>& a, const std::shared_ptr<ExecStatus>& b) {
+  auto watched = [](const std::shared_ptr<ExecStatus>& s) { return s && s->before && s->after; };
+  if (!watched(a) || a == b) return b;
+  if (!watched(b)) return a;
+  const auto &front = a->first <= b->first ? a : b, &back = a->last >= b->last ? a : b;
+  auto s = std::make_shared<ExecStatus>();
+  s->before = front->before;
+  s->first = front->first;
+  s->after = back->after;
+  s->last = back->last;
+  return s;
 }
 
 // In front of a change of `b` on the compute stream, and behind it.
@@ -3116,7 +3140,7 @@ b200_error* b200_cache_write_pages(b200_client* c, b200_buffer* cache, b200_buff
   int launches = 0;
   CUDA_TRY(launch_write_pages(shape, cache->ptr, rows->ptr, slots, (long long)n, c->compute, &launches));
   // an execution that gave up on a wait left its mark on the rows: what was made of them carries it too
-  if (rows->status && !(cache->status && cache->status->failed())) cache->status = rows->status;
+  cache->status = both_statuses(cache->status, rows->status);
   return after_change(c, cache, launches);
 } catch (const std::exception& e) {
   return make_error(B200_INTERNAL, std::string("write_pages: ") + e.what());

@@ -29,6 +29,64 @@ __device__ __forceinline__ int length_of(const Prompt& a, int b) {
   return a.lengths ? min(max(a.lengths[b], 0), a.tokens) : a.tokens;
 }
 
+// Whether a position is seen; the keys' and values' sums run over these.
+__device__ __forceinline__ bool sees(const Prompt& a, int row, int key) {
+  return key <= row && (a.window == 0 || row - key < a.window || key < a.sinks);
+}
+
+// The kernels multiply whole tiles of values by weights that are zero where a row does not look, and zero times an infinity or a NaN is
+// none. They notice by a result that is no finite number, and then this has another look at such rows, a warp at each: where a value
+// that the row does not see, but that lay in a tile with what it does, is no finite number, the row is made again from what it sees
+// alone. Nothing is spent on it otherwise; the rows of a tile that a prompt's own infinities reach take some fifty times as long.
+constexpr int kReach = 384;           // positions beside its own and beside its window that a row's tiles cover, two tiles of queries together
+template <typename T>
+__device__ __noinline__ void mend_rows(const Prompt& a, int b, int h, int q0, int rows, int warp, int warps) {
+  const int lane = threadIdx.x & 31, D = a.dim, n = length_of(a, b), kvh = h / a.group;
+  const long long stride = (long long)a.kv_heads * D, base = ((long long)b * a.tokens * a.kv_heads + kvh) * D;
+  const T *keys = (const T*)a.k + base, *values = (const T*)a.v + base;
+  auto finite = [](T v) { return fabsf(to_float(v)) <= 3.4028235e38f; };
+  for (int row = q0 + warp; row < min(q0 + rows, n); row += warps) {
+    const long long at = (((long long)b * a.tokens + row) * a.heads + h) * D;
+    T* out = (T*)a.out + at;
+    bool odd = false;
+    for (int d = lane; d < D; d += 32) odd |= !finite(out[d]);
+    if (!__any_sync(0xFFFFFFFFu, odd)) continue;
+    auto hidden = [&](int from, int to) {                          // whether one of these is hidden and not finite
+      bool found = false;
+      for (int key = max(from, 0); key < min(to, n); ++key)
+        if (!sees(a, row, key))
+          for (int d = lane; d < D; d += 32) found |= !finite(values[key * stride + d]);
+      return __any_sync(0xFFFFFFFFu, found);
+    };
+    const int start = a.window > 0 ? max(0, row - a.window + 1) : 0, sinks = min(a.sinks, start);
+    if (!hidden(row + 1, row + kReach) && !hidden(start - kReach, start) && !hidden(sinks, sinks + kReach)) continue;
+    float q[8], o[8], m = neg_inf(), l = 0.f;                      // features lane, lane + 32, ...
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      q[e] = lane + 32 * e < D ? to_float(((const T*)a.q)[at + lane + 32 * e]) * a.scale : 0.f;
+      o[e] = 0.f;
+    }
+    for (int i = 0; i < sinks + row - start + 1; ++i) {
+      const long long key = (i < sinks ? i : start + i - sinks) * stride;
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (lane + 32 * e < D) s = fmaf(q[e], to_float(keys[key + lane + 32 * e]), s);
+      s = warp_sum(s);
+      const float top = fmaxf(m, s), ref = top == neg_inf() ? 0.f : top, keep = exp2f(m - ref), p = exp2f(s - ref);
+      m = top;
+      l = l * keep + p;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (lane + 32 * e < D) o[e] = fmaf(p, to_float(values[key + lane + 32 * e]), o[e] * keep);
+    }
+    const bool some = l > 0.f || l != l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (lane + 32 * e < D) out[lane + 32 * e] = from_float<T>(some ? o[e] / l : 0.f);
+  }
+}
+
 // 32-bit data on the FMA pipe: a block takes 64 queries of a head, in tiles of 64 keys. A thread holds 4 x 4 scores and, of the
 // outputs, four rows and every sixteenth group of four features.
 constexpr int kTile = 64, kScoreRow = kTile + 4;
@@ -96,8 +154,7 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const __grid_constant__
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int key = k0 + tx + 16 * j;
-          const bool see = key <= row && key < n && (a.window == 0 || row - key < a.window || key < a.sinks);
-          if (!see) s[i][j] = neg_inf();
+          if (key >= n || !sees(a, row, key)) s[i][j] = neg_inf();
           top = fmaxf(top, s[i][j]);
         }
 #pragma unroll
@@ -146,6 +203,7 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const __grid_constant__
       __syncwarp();
     }
   }
+  float odd = 0.f;                                                  // NaN where a result is not finite
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = q0 + ty * 4 + i;
@@ -157,9 +215,14 @@ __global__ void __launch_bounds__(256) prompt_fma_kernel(const __grid_constant__
       const int d = (tx + 16 * c) * 4;
       if (d < D)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) to[d + e] = from_float<T>(some ? o[i][c][e] / l[i] : 0.f);
+        for (int e = 0; e < 4; ++e) {
+          const float v = row < n ? o[i][c][e] : 0.f;
+          odd = fmaf(v, 0.f, odd);
+          to[d + e] = from_float<T>(some ? v / l[i] : 0.f);
+        }
     }
   }
+  if (__syncthreads_or(odd != odd)) mend_rows<T>(a, b, h, q0, kTile, tid >> 5, 8);
 }
 
 // ---- 16-bit data on the tensor cores -------------------------------------------------------------------
@@ -318,10 +381,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid
   // of a tile have all products so far, have been read; both threads of a row have spoken; nothing is under way
   constexpr int Q_FULL = 0, Q_EMPTY = 1, K_FULL = 2, K_EMPTY = K_FULL + S, V_FULL = K_EMPTY + S, V_EMPTY = V_FULL + S, S_FULL = V_EMPTY + S, P_FULL = S_FULL + 2,
                 PV_DONE = P_FULL + 4, O_EMPTY = PV_DONE + 2, AGREED = O_EMPTY + 2, DRAINED = AGREED + 4, BARRIERS = DRAINED + 1;
-  static_assert(BARRIERS * 8 + 8 <= 512, "barriers");
+  static_assert(BARRIERS * 8 + 12 <= 512, "barriers");
   auto bar = [base = smem_u32(bars)](int k) { return base + 8u * (uint32_t)k; };
   uint32_t* tmem_slot = (uint32_t*)(bars + BARRIERS);
-  volatile int* failed = (volatile int*)(tmem_slot + 1);
+  volatile int *failed = (volatile int*)(tmem_slot + 1), *strange = failed + 1;
   float* said = (float*)((uint8_t*)bars + 512);                      // [parity][half][row]
   uint8_t* stage = (uint8_t*)(said + 4 * kRows);                     // [warp][row][32 results]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, D = a.dim;
@@ -329,6 +392,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid
     for (int k = 0; k < BARRIERS; ++k)
       mbar_init(bar(k), k >= P_FULL && k < PV_DONE ? 4 : k >= O_EMPTY && k < AGREED ? 8 / ITEMS : k >= AGREED && k < DRAINED ? 2 : 1);
     *failed = 0;
+    *strange = 0;                                                    // whether a result is not finite
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 9) {
@@ -608,6 +672,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid
       }
       const bool some = w.count && row < w.n;
       const float inv = some && (l > 0.f || l != l) ? 1.f / l : 0.f;
+      uint64_t odd = 0;                                              // NaN where one is not finite
 #pragma unroll
       for (int c0 = 0; c0 < (ITEMS == 2 ? DP : DP / 2); c0 += 32) {
         const int c = (ITEMS == 2 ? 0 : half * (DP / 2)) + c0;
@@ -616,6 +681,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid
           load32(outputs(u) + mine + c, o);
           loaded();
           settle(o);
+          if (some) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) odd = fma2(two(o[e], o[e + 1]), two(0.f, 0.f), odd);
+          }
         }
         // by way of shared memory, so that a store touches eight rows' 64 bytes and not 32 rows' 16: those took 8600 cycles a tile, 4500 so, most of it
         // the wait for the last product
@@ -639,6 +708,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid
         }
         __syncwarp();
       }
+      if (first(odd) != first(odd) || second(odd) != second(odd)) *strange = 1;
       if (w.count) {
         before_sync();
         __syncwarp();
@@ -650,6 +720,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid
   __syncthreads();
   if (tid == 0 && *failed) atomicAdd(error_flag, 1);
   if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (!*strange || *failed) return;
+  for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+    const Unit<ITEMS> w(a, unit);
+#pragma unroll 1
+    for (int u = 0; u < ITEMS; ++u) mend_rows<T>(a, w.b, w.head[u], w.q0[u], kRows, warp, kMmaThreads / 32);
+  }
 }
 
 size_t fma_smem(int dim) { return (size_t)(3 * kTile * (dim + 4) + kTile * kScoreRow) * 4; }

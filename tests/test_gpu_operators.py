@@ -8,6 +8,7 @@ bits for the second product: u mag more, or u^2 mag where they go in two pieces.
 import numpy as np
 import pytest
 
+import b200
 from b200.pages import PagedCache
 from b200.shlo.builder import Builder
 from oracle import interp, operators
@@ -152,6 +153,19 @@ def test_paged_attention_scores_at_the_edge(client):
     assert np.isnan(got[0]).all() and np.isfinite(got[1]).all()
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_paged_attention_many_small_weights_beside_a_large_one(client, dt):
+    """60000 positions of e^-17 each, which are 2.5e-3 of the result together, beside one whose value is zero."""
+    n, S, D = 60001, 64, 64
+    pages = -(-n // S)
+    q, cache = np.zeros((1, 1, D)), np.zeros((1, 2, pages, S, 1, D))
+    q[..., 0], cache[0, 0, 5, 3, 0, 0] = 17.0, 1.0
+    cache[0, 1] = 1.0
+    cache[0, 1, 5, 3] = 0.0
+    table = np.arange(pages, dtype=np.int32)[None]
+    check_paged(client, q, cache, table, np.array([n], np.int32), None, dt, scale=1.0)
+
+
 def test_paged_attention_of_nothing(client):
     for B, W in ((0, 3), (2, 0)):
         q, cache = np.ones((B, 2, 8), np.float32), np.ones((1, 2, 0 if W == 0 else 4, 2, 1, 8), np.float32)
@@ -207,6 +221,32 @@ def test_window_attention_padded_batch(client, dt):
         n = min(max(n, 0), 150)
         q[b, n:], k[b, n:], v[b, n:] = np.nan, np.inf, np.nan          # nobody reads what stands behind a sequence
     check_prompt(client, q, k, v, lengths, dt, window=70, sinks=2, scale=0.2)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,H,KH,D,window,sinks", [(1, 2, 1, 64, 0, 0), (1, 2, 1, 64, 40, 3), (1, 1, 1, 256, 150, 20), (4, 32, 8, 64, 40, 3), (4, 32, 32, 128, 0, 0), (5, 32, 32, 64, 130, 129)])
+def test_window_attention_of_values_that_are_no_numbers(client, dt, B, H, KH, D, window, sinks):
+    """Infinities and NaN in keys and values reach the rows that see them and no other, in all forms of the kernels (one tile of queries a
+    block, two of one head, two heads)."""
+    T = 300
+    rng = np.random.default_rng(B * D + window)
+    q, k, v = prompt_case(rng, B, T, H, KH, D, dt)
+    lengths = np.array([300, 299, 131, 140, 0], np.int32)[:B]
+    v[0, 130], v[:, 250, :, 3], v[:, 255], k[:, 298] = np.inf, np.nan, -np.inf, np.nan
+    args, dts = [q, k, v, lengths], [dt] * 3 + ["i32"]
+    got = run(client, lambda b, *a: b.window_attention(*a, window=window, sinks=sinks), args, dts)[0]
+    kw = dict(lengths=lengths, window=window, sinks=sinks)
+    heads = [0, 1, H - 1]
+    for h in sorted(set(x for x in heads if x < H)):
+        g = h // (H // KH)
+        one = [q[:, :, h:h + 1], k[:, :, g:g + 1], v[:, :, g:g + 1]]
+        with np.errstate(all="ignore"):
+            raw = operators.window_attention(*one, **kw)
+            want, mag, top = operators.window_attention(*[np.where(np.isfinite(t), t, 0.0) for t in one], bounds=True, **kw)
+        fine = np.isfinite(raw)
+        np.testing.assert_array_equal(np.isfinite(got[:, :, h:h + 1]), fine)
+        tol = attention_tolerance(want, mag, top, T, D, dt, 0.0 if dt == "f32" else U[dt])
+        assert (np.abs(got[:, :, h:h + 1] - want)[fine] <= tol[fine]).all()
 
 
 # ---- log probabilities ---------------------------------------------------------------------------------
@@ -436,6 +476,29 @@ def test_moves_keep_their_place_among_executions_and_reads(client):
         np.testing.assert_array_equal(buf.to_numpy(), new)
         np.testing.assert_array_equal(before.to_numpy(), 2 * old)
         np.testing.assert_array_equal(behind.to_numpy(), 2 * new)
+
+
+def test_moves_keep_what_an_execution_reported(client):
+    """Rows of an execution that gave up on a wait (test hook: a barrier nothing arrives at) make the cache's contents invalid, and rows of
+    a good one written behind them do not hide it."""
+    shape = (1, 2, 4, 1, 256)
+    cache = client.buffer_from_host(np.zeros((1, 2, 2, 4, 1, 256), np.float32))
+    b = Builder()
+    x = b.arg((256, 256), "f32")
+    exe = client.compile(b.module([b.reshape(b.slice(b.dot_general(x, x, ([1], [0])), (0, 0), (8, 256)), shape)]))
+    arg = client.buffer_from_host(np.eye(256, dtype=np.float32))
+    client.synchronize()
+    client.debug_arm_wait_expiry(1000)
+    bad, good = (exe.execute([arg])[0] for _ in range(2))
+    client.write_pages(cache, bad, [0, 1, 2, 3])
+    client.write_pages(cache, good, [4, 5, 6, 7])
+    with pytest.raises(b200.B200Error, match="bounded"):
+        cache.to_numpy()
+    with pytest.raises(b200.B200Error):
+        client.synchronize()
+    other = client.buffer_from_host(np.zeros((1, 2, 2, 4, 1, 256), np.float32))
+    client.write_pages(other, good, [4, 5, 6, 7])
+    assert np.array_equal(other.to_numpy()[0, :, 1, :, 0], np.eye(256, dtype=np.float32)[:8].reshape(2, 4, 256))
 
 
 def test_cache_of_more_than_32_bits(client):

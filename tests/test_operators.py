@@ -226,3 +226,11 @@ def test_paged_cache_refuses():
 def test_indices_are_whole_numbers_of_32_bits(values, ndim):
     with pytest.raises(b200.B200Error):
         b200._indices(values, ndim)
+
+
+@pytest.mark.parametrize("value", ["0x7F800000 : f32", "0x3F000000 : f32", "nan : f32", "\"large\"", "1.0e+99 : f64"])
+def test_scales_that_are_no_numbers(value):
+    text = paged_text(scale=0.5)
+    assert "scale = 5.000000000e-01 : f32" in text
+    with pytest.raises(b200.B200Error, match="scale"):
+        b200.compile_to_plan(text.replace("5.000000000e-01 : f32", value))
