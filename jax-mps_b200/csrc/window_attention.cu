@@ -29,6 +29,12 @@ __device__ __forceinline__ int length_of(const Prompt& a, int b) {
   return a.lengths ? min(max(a.lengths[b], 0), a.tokens) : a.tokens;
 }
 
+__device__ __forceinline__ float power(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // Whether a position is seen; the keys' and values' sums run over these.
 __device__ __forceinline__ bool sees(const Prompt& a, int row, int key) {
   return key <= row && (a.window == 0 || row - key < a.window || key < a.sinks);
@@ -36,11 +42,11 @@ __device__ __forceinline__ bool sees(const Prompt& a, int row, int key) {
 
 // The kernels multiply whole tiles of values by weights that are zero where a row does not look, and zero times an infinity or a NaN is
 // none. They notice by a result that is no finite number, and then this has another look at such rows, a warp at each: where a value
-// that the row does not see, but that lay in a tile with what it does, is no finite number, the row is made again from what it sees
-// alone. Nothing is spent on it otherwise; the rows of a tile that a prompt's own infinities reach take some fifty times as long.
+// that the row does not see, but that lay in a tile with what it does, is no finite number (or where `all` asks for it), the row is made
+// again from what it sees alone. Nothing is spent on it otherwise; the rows of a tile that a prompt's own infinities reach take some fifty times as long.
 constexpr int kReach = 384;           // positions beside its own and beside its window that a row's tiles cover, two tiles of queries together
 template <typename T>
-__device__ __noinline__ void mend_rows(const Prompt& a, int b, int h, int q0, int rows, int warp, int warps) {
+__device__ __noinline__ void mend_rows(const Prompt& a, int b, int h, int q0, int rows, int warp, int warps, bool all) {
   const int lane = threadIdx.x & 31, D = a.dim, n = length_of(a, b), kvh = h / a.group;
   const long long stride = (long long)a.kv_heads * D, base = ((long long)b * a.tokens * a.kv_heads + kvh) * D;
   const T *keys = (const T*)a.k + base, *values = (const T*)a.v + base;
@@ -59,7 +65,7 @@ __device__ __noinline__ void mend_rows(const Prompt& a, int b, int h, int q0, in
       return __any_sync(0xFFFFFFFFu, found);
     };
     const int start = a.window > 0 ? max(0, row - a.window + 1) : 0, sinks = min(a.sinks, start);
-    if (!hidden(row + 1, row + kReach) && !hidden(start - kReach, start) && !hidden(sinks, sinks + kReach)) continue;
+    if (!all && !hidden(row + 1, row + kReach) && !hidden(start - kReach, start) && !hidden(sinks, sinks + kReach)) continue;
     float q[8], o[8], m = neg_inf(), l = 0.f;                      // features lane, lane + 32, ...
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -73,7 +79,7 @@ __device__ __noinline__ void mend_rows(const Prompt& a, int b, int h, int q0, in
       for (int e = 0; e < 8; ++e)
         if (lane + 32 * e < D) s = fmaf(q[e], to_float(keys[key + lane + 32 * e]), s);
       s = warp_sum(s);
-      const float top = fmaxf(m, s), ref = top == neg_inf() ? 0.f : top, keep = exp2f(m - ref), p = exp2f(s - ref);
+      const float top = fmaxf(m, s), ref = top == neg_inf() ? 0.f : top, keep = power(m - ref), p = power(s - ref);
       m = top;
       l = l * keep + p;
 #pragma unroll
@@ -87,142 +93,249 @@ __device__ __noinline__ void mend_rows(const Prompt& a, int b, int h, int q0, in
   }
 }
 
-// 32-bit data on the FMA pipe: a block takes 64 queries of a head, in tiles of 64 keys. A thread holds 4 x 4 scores and, of the
-// outputs, four rows and every sixteenth group of four features.
-constexpr int kTile = 64, kScoreRow = kTile + 4;
+// ---- 32-bit data ---------------------------------------------------------------------------------------
+// A block takes 64 queries of a head, a warp 16 of them, and goes through 32 places of its row of keys at a time: first the sinks that lie
+// in front of its first query's window, then from that window's first key on, whichever key that is, so that no tile is half empty. Keys
+// and values come by cp.async, a tile ahead. Both products run on the tensor cores by mma.sync (tf32 m16n8k8) in three parts, hi hi + hi
+// lo + lo hi, hi a word rounded to the 19 bits that they read and lo what that leaves, rounded likewise; a tile's outputs are added up apart
+// and then to the others in 32 bits, since the tensor core cuts its sums. The order of the features within a step of 16 and of the keys
+// within a step of 8 is chosen so that fragments are loaded 16 bytes a thread, free of bank conflicts, and so that the scores' fragments
+// are the weights'.
+constexpr int kWideThreads = 128;
+template <int DP>
+struct Wide {
+  // warps that share their queries, each with its own 32 keys of a tile: two where the tiles leave room for it
+  static constexpr int HALVES = DP == 64 ? 2 : 1, ROWS = 64 / HALVES, KEYS = 32 * HALVES;
+  static constexpr int KP = DP + 16, VP = DP + 4;                    // floats between rows of queries and keys, of values
+  static constexpr int STAGE = KEYS * (KP + VP), SMEM = (ROWS * KP + 2 * STAGE) * 4;
+  static constexpr int PER_SM = DP <= 128 ? 2 : 1;
+  static constexpr bool HELD = DP == 64;                             // the queries' parts stay in registers
+  static_assert(HALVES == 1 || ROWS * (DP + 2) <= STAGE, "no room for the halves' outputs");
+  static_assert((SMEM + 1024) * PER_SM <= 233472, "more than an SM has");
+};
 
-template <typename T>
-__global__ void __launch_bounds__(256) prompt_fma_kernel(const __grid_constant__ Prompt a) {
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void halves(float v, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(v));
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(v - __uint_as_float(hi)));
+}
+// c[j] += a b[j] for four products side by side: one behind another each would wait for the last.
+__device__ __forceinline__ void mma_four(float (&c)[4][4], const uint32_t (&hi)[4], const uint32_t (&lo)[4], const float (&b0)[4], const float (&b1)[4]) {
+  uint32_t h0[4], l0[4], h1[4], l1[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { halves(b0[j], h0[j], l0[j]); halves(b1[j], h1[j], l1[j]); }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) mma_tf32(c[j], lo, h0[j], h1[j]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) mma_tf32(c[j], hi, l0[j], l1[j]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) mma_tf32(c[j], hi, h0[j], h1[j]);
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kWideThreads, Wide<DP>::PER_SM) prompt_wide_kernel(const __grid_constant__ Prompt a) {
   pdl_prologue();
+  using C = Wide<DP>;
+  constexpr int P = DP / 4, KEYS = C::KEYS;
   extern __shared__ __align__(16) float smem[];
-  const int D = a.dim, P = D + 4, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  float *qs = smem, *ks = qs + kTile * P, *vs = ks + kTile * P, *ss = vs + kTile * P;
+  const int D = a.dim, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane / 4, t = lane % 4, half = warp % C::HALVES, rows = warp / C::HALVES * 16;
   const int h = blockIdx.y, b = blockIdx.z, kvh = h / a.group, n = length_of(a, b);
-  const int q0 = (int)(gridDim.x - 1 - blockIdx.x) * kTile;         // the rows that see most go first
-  constexpr int N = Pack<T>::N;
-  const int pieces = D / N;
-  auto load = [&](float* to, const void* from, int row0, int heads, int head, float scale) {
-    for (int i = tid; i < kTile * pieces; i += 256) {
-      const int row = i / pieces, c = i % pieces * N;
-      uint4 v = {0, 0, 0, 0};
-      if (row0 + row < n) v = *(const uint4*)((const T*)from + (((long long)b * a.tokens + row0 + row) * heads + head) * D + c);
-      float f[N];
-      unpack<T>(v, f);
-#pragma unroll
-      for (int e = 0; e < N; ++e) to[row * P + c + e] = f[e] * scale;
-    }
+  const int q0 = (int)(gridDim.x - 1 - blockIdx.x) * C::ROWS, row0 = q0 + rows;           // the rows that see most go first
+  const int start = a.window > 0 ? max(0, q0 - a.window + 1) : 0, sinks = min(a.sinks, start), shift = start - sinks;
+  const int places = q0 < n ? sinks + min(q0 + C::ROWS, n) - start : 0, tiles = (places + KEYS - 1) / KEYS;
+  float *qs = smem, *stages = qs + C::ROWS * C::KP;
+  auto copy = [&](float* to, const float* from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(there ? 16 : 0) : "memory");
   };
-  float m[4], l[4], o[4][4][4];                                     // row, group of features, feature
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    m[i] = neg_inf();
-    l[i] = 0.f;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][c][e] = 0.f;
+  // a thread copies the same four features of every so many rows
+  const int c0 = tid % P * 4, r0 = tid / P;
+  const long long stride = (long long)a.kv_heads * D, base = ((long long)b * a.tokens * a.kv_heads + kvh) * D + c0;
+  auto fetch = [&](int tile) {
+    if (tile < tiles) {
+      float *ks = stages + (tile & 1) * C::STAGE + r0 * C::KP + c0, *vs = stages + (tile & 1) * C::STAGE + KEYS * C::KP + r0 * C::VP + c0;
+#pragma unroll 8
+      for (int r = 0; r < KEYS; r += kWideThreads / P) {
+        const int place = tile * KEYS + r0 + r;
+        const bool there = place < places && c0 < D;
+        const long long at = there ? base + (place + (place < sinks ? 0 : shift)) * stride : 0;
+        copy(ks + r * C::KP, (const float*)a.k + at, there);
+        copy(vs + r * C::VP, (const float*)a.v + at, there);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (tiles) {
+    for (int r = r0; r < C::ROWS; r += kWideThreads / P) {
+      const bool there = q0 + r < n && c0 < D;
+      copy(qs + r * C::KP + c0, (const float*)a.q + (there ? (((long long)b * a.tokens + q0 + r) * a.heads + h) * D + c0 : 0), there);
+    }
   }
-  if (q0 < n) {
-    load(qs, a.q, q0, a.heads, h, a.scale);
-    const int last = min(q0 + kTile, n), first = a.window > 0 ? max(0, q0 - a.window + 1) : 0;
-    for (int k0 = 0; k0 < last; k0 += kTile) {
-      if (k0 + kTile <= first && k0 >= a.sinks) continue;
-      __syncthreads();
-      load(ks, a.k, k0, a.kv_heads, kvh, 1.f);
-      load(vs, a.v, k0, a.kv_heads, kvh, 1.f);
-      __syncthreads();
-      float s[4][4];
+  fetch(0);
+  float m[2] = {neg_inf(), neg_inf()}, l[2] = {0.f, 0.f}, o[DP / 32][4][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+  for (int c = 0; c < DP / 32; ++c)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-      for (int d = 0; d < D; d += 4) {
-        float4 q[4], k[4];
+    for (int e = 0; e < 4; ++e) o[c][e][0] = o[c][e][1] = o[c][e][2] = o[c][e][3] = 0.f;
+  // the queries of 16 features, two steps of a product
+  auto queries = [&](int c, uint32_t (&hi)[2][4], uint32_t (&lo)[2][4]) {
+    const float4 x = *(const float4*)(qs + (rows + g) * C::KP + c * 16 + t * 4), y = *(const float4*)(qs + (rows + g + 8) * C::KP + c * 16 + t * 4);
+    halves(x.x, hi[0][0], lo[0][0]); halves(y.x, hi[0][1], lo[0][1]); halves(x.y, hi[0][2], lo[0][2]); halves(y.y, hi[0][3], lo[0][3]);
+    halves(x.z, hi[1][0], lo[1][0]); halves(y.z, hi[1][1], lo[1][1]); halves(x.w, hi[1][2], lo[1][2]); halves(y.w, hi[1][3], lo[1][3]);
+  };
+  uint32_t qh[C::HELD ? DP / 16 : 1][2][4], ql[C::HELD ? DP / 16 : 1][2][4];
+  if (C::HELD && tiles) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = *(const float4*)(qs + (ty * 4 + i) * P + d);
+    for (int c = 0; c < (C::HELD ? DP / 16 : 1); ++c) queries(c, qh[c], ql[c]);
+  }
+#pragma unroll 1
+  for (int tile = 0; tile < tiles; ++tile) {
+    fetch(tile + 1);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncthreads();
+    const float *ks = stages + (tile & 1) * C::STAGE + half * 32 * C::KP, *vs = stages + (tile & 1) * C::STAGE + KEYS * C::KP + half * 32 * C::VP;
+    // the keys of the tile: its sinks, then from `low` to `high`
+    const int p0 = tile * KEYS + half * 32, low = max(p0, sinks) + shift, high = p0 + 31 + shift;
+    const bool some_sinks = p0 < sinks, hidden = low > row0 + 15 || (a.window > 0 && row0 - high >= a.window && low >= a.sinks);
+    if (some_sinks || !hidden) {
+      float s[4][4] = {};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) k[j] = *(const float4*)(ks + (tx + 16 * j) * P + d);
+      for (int c = 0; c < DP / 16; ++c)
+        if (c * 16 < D) {
+          if (!C::HELD) queries(c, qh[0], ql[0]);
+          const int at = C::HELD ? c : 0;
+          float k[4][4], add[4][4] = {};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[i][j] = fmaf(q[i].x, k[j].x, fmaf(q[i].y, k[j].y, fmaf(q[i].z, k[j].z, fmaf(q[i].w, k[j].w, s[i][j]))));
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = q0 + ty * 4 + i;
-        float top = neg_inf();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int key = k0 + tx + 16 * j;
-          if (key >= n || !sees(a, row, key)) s[i][j] = neg_inf();
-          top = fmaxf(top, s[i][j]);
-        }
-#pragma unroll
-        for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-        const float now = fmaxf(m[i], top), ref = now == neg_inf() ? 0.f : now, keep = exp2f(m[i] - ref);
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float p = exp2f(s[i][j] - ref);
-          sum += p;
-          ss[(ty * 4 + i) * kScoreRow + tx + 16 * j] = p;
-        }
-#pragma unroll
-        for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
-        l[i] = l[i] * keep + sum;
-        m[i] = now;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[i][c][e] *= keep;
-      }
-      __syncwarp();                                                 // a row's scores stay within a warp
-      for (int t = 0; t < kTile; t += 4) {
-        float4 p[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = *(const float4*)(ss + (ty * 4 + i) * kScoreRow + t);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int d = (tx + 16 * c) * 4;
-          if (d < D) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const float4 v = *(const float4*)(vs + (t + u) * P + d);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float w = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
-                o[i][c][0] = fmaf(w, v.x, o[i][c][0]);
-                o[i][c][1] = fmaf(w, v.y, o[i][c][1]);
-                o[i][c][2] = fmaf(w, v.z, o[i][c][2]);
-                o[i][c][3] = fmaf(w, v.w, o[i][c][3]);
-              }
-            }
+          for (int j = 0; j < 4; ++j) {
+            const float4 v = *(const float4*)(ks + (j * 8 + g) * C::KP + c * 16 + t * 4);
+            k[0][j] = v.x; k[1][j] = v.y; k[2][j] = v.z; k[3][j] = v.w;
           }
+          mma_four(add, qh[at][0], ql[at][0], k[0], k[1]);
+          mma_four(add, qh[at][1], ql[at][1], k[2], k[3]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[j][i] += add[j][i];
+        }
+      const bool edge = high > row0 || (a.window > 0 && row0 + 15 - low >= a.window);
+      float top[2] = {neg_inf(), neg_inf()};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[j][i] *= a.scale;
+          if (edge) {
+            const int place = p0 + j * 8 + t * 2 + (i & 1);
+            if (!sees(a, row0 + g + i / 2 * 8, place + (place < sinks ? 0 : shift))) s[j][i] = neg_inf();
+          }
+          top[i / 2] = fmaxf(top[i / 2], s[j][i]);
+        }
+      uint32_t hi[4][4], lo[4][4];
+      float keep[2], ref[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 1));
+        top[r] = fmaxf(fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 2)), m[r]);
+        ref[r] = top[r] == neg_inf() ? 0.f : top[r];
+        keep[r] = power(m[r] - ref[r]);
+        l[r] *= keep[r];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[i] = power(s[j][i] - ref[i / 2]);
+          l[i / 2] += p[i];
+          halves(p[i], hi[j][(i & 1) * 2 + i / 2], lo[j][(i & 1) * 2 + i / 2]);
         }
       }
-      __syncwarp();
+      if (__any_sync(0xFFFFFFFFu, top[0] > m[0] || top[1] > m[1])) {
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[c][e][i] *= keep[i / 2];
+      }
+      m[0] = top[0];
+      m[1] = top[1];
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c)
+        if (c * 32 < D) {
+          float add[4][4] = {};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float4 x = *(const float4*)(vs + (j * 8 + t * 2) * C::VP + c * 32 + g * 4), y = *(const float4*)(vs + (j * 8 + t * 2 + 1) * C::VP + c * 32 + g * 4);
+            const float v0[4] = {x.x, x.y, x.z, x.w}, v1[4] = {y.x, y.y, y.z, y.w};
+            mma_four(add, hi[j], lo[j], v0, v1);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[c][e][i] += add[e][i];
+        }
+    }
+    __syncthreads();                                                // the tile's place may be filled again
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
+  }
+  if (C::HALVES == 2 && tiles) {                                     // the second half's outputs to the first: a lane's own words, 16 warps' apart
+    float* at = stages + warp / 2 * (16 * (DP + 2)) + lane;
+    if (half) {
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) at[(c * 16 + i) * 32] = o[c][i / 4][i % 4];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        if (t < 2) at[(DP / 2) * 32 - lane + (g + 8 * r) * 2 + t] = t ? l[r] : m[r];
+    }
+    __syncthreads();
+    if (!half) {
+      float mine[2], other[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float* stats = at - lane + (DP / 2) * 32 + (g + 8 * r) * 2;
+        const float top = fmaxf(m[r], stats[0]), ref = top == neg_inf() ? 0.f : top;
+        mine[r] = power(m[r] - ref);
+        other[r] = power(stats[0] - ref);
+        l[r] = l[r] * mine[r] + stats[1] * other[r];
+      }
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[c][i / 4][i % 4] = o[c][i / 4][i % 4] * mine[i % 4 / 2] + at[(c * 16 + i) * 32] * other[i % 4 / 2];
     }
   }
   float odd = 0.f;                                                  // NaN where a result is not finite
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = q0 + ty * 4 + i;
-    if (row >= a.tokens) continue;
-    const bool some = row < n && (l[i] > 0.f || l[i] != l[i]);
-    T* to = (T*)a.out + (((long long)b * a.tokens + row) * a.heads + h) * D;
+  for (int r = 0; r < 2; ++r) {
+    const int row = row0 + g + r * 8;
+    if (half || row >= a.tokens) continue;
+    const float inv = row < n && (l[r] > 0.f || l[r] != l[r]) ? 1.f / l[r] : 0.f;
+    float* to = (float*)a.out + (((long long)b * a.tokens + row) * a.heads + h) * D + t * 8;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int d = (tx + 16 * c) * 4;
-      if (d < D)
+    for (int c = 0; c < DP / 32; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = row < n ? o[i][c][e] : 0.f;
-          odd = fmaf(v, 0.f, odd);
-          to[d + e] = from_float<T>(some ? v / l[i] : 0.f);
-        }
-    }
+      for (int i = 0; i < 2; ++i) {
+        if (c * 32 + t * 8 >= D) continue;
+        float4 v = {0.f, 0.f, 0.f, 0.f};
+        if (row < n) v = {o[c][0][r * 2 + i] * inv, o[c][1][r * 2 + i] * inv, o[c][2][r * 2 + i] * inv, o[c][3][r * 2 + i] * inv};
+        odd = fmaf(v.x + v.y + v.z + v.w, 0.f, odd);
+        *(float4*)(to + c * 32 + i * 4) = v;
+      }
   }
-  if (__syncthreads_or(odd != odd)) mend_rows<T>(a, b, h, q0, kTile, tid >> 5, 8);
+  // (with all rows that are not finite: parts of infinities are no numbers)
+  if (__syncthreads_or(odd != odd)) mend_rows<float>(a, b, h, q0, C::ROWS, warp, kWideThreads / 32, true);
 }
 
 // ---- 16-bit data on the tensor cores -------------------------------------------------------------------
@@ -316,12 +429,6 @@ __device__ __forceinline__ uint32_t pair16(float lo, float hi) {
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
-__device__ __forceinline__ float power(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -724,18 +831,16 @@ __global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid
   for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
     const Unit<ITEMS> w(a, unit);
 #pragma unroll 1
-    for (int u = 0; u < ITEMS; ++u) mend_rows<T>(a, w.b, w.head[u], w.q0[u], kRows, warp, kMmaThreads / 32);
+    for (int u = 0; u < ITEMS; ++u) mend_rows<T>(a, w.b, w.head[u], w.q0[u], kRows, warp, kMmaThreads / 32, false);
   }
 }
 
-size_t fma_smem(int dim) { return (size_t)(3 * kTile * (dim + 4) + kTile * kScoreRow) * 4; }
-
-template <typename T>
-cudaError_t launch_fma(const Prompt& a, cudaStream_t stream, int* launches) {
+template <int DP>
+cudaError_t launch_wide(const Prompt& a, cudaStream_t stream, int* launches) {
   static bool done[64] = {};
-  if (cudaError_t e = allow_smem(prompt_fma_kernel<T>, fma_smem(256), done)) return e;
-  return launch_op(prompt_fma_kernel<T>, dim3((unsigned)((a.tokens + kTile - 1) / kTile), (unsigned)a.heads, (unsigned)a.batch), 256, fma_smem(a.dim),
-                   stream, launches, a);
+  if (cudaError_t e = allow_smem(prompt_wide_kernel<DP>, Wide<DP>::SMEM, done)) return e;
+  return launch_op(prompt_wide_kernel<DP>, dim3((unsigned)((a.tokens + Wide<DP>::ROWS - 1) / Wide<DP>::ROWS), (unsigned)a.heads, (unsigned)a.batch), kWideThreads,
+                   Wide<DP>::SMEM, stream, launches, a);
 }
 
 template <typename T, int DP, int ITEMS>
@@ -776,7 +881,7 @@ cudaError_t launch_16bit(const Prompt& a, int* error_flag, cudaStream_t stream, 
 
 const char* window_attention_plan(OperatorLaunch& op) {
   if (op.heads > 65535 || op.batch > 65535) return "more than 65535 heads or sequences";
-  if (op.tokens > 65535 * kTile) return "prompts of more than 65535 tiles of 64 tokens";
+  if (op.tokens >= (1 << 30)) return "prompts of 2^30 tokens and more";
   if ((long long)op.batch * op.tokens >= (1LL << 31)) return "2^31 tokens and more";
   if ((long long)op.batch * op.heads * ((op.tokens + kRows - 1) / kRows) >= (1LL << 31) - kSMs) return "too many heads and sequences";
   op.scratch_bytes = 0;
@@ -796,7 +901,8 @@ cudaError_t launch_window_attention(const OperatorLaunch& op, void* const* args,
   a.batch = op.batch; a.tokens = op.tokens; a.heads = op.heads; a.kv_heads = op.kv_heads; a.dim = op.dim; a.group = op.heads / op.kv_heads;
   a.window = op.window; a.sinks = op.sinks;
   a.scale = op.scale * kLog2e;
-  if (op.type == 0) return launch_fma<float>(a, stream, launches);
+  if (op.type == 0)
+    return op.dim <= 64 ? launch_wide<64>(a, stream, launches) : op.dim <= 128 ? launch_wide<128>(a, stream, launches) : launch_wide<256>(a, stream, launches);
   if (op.type == 1) return launch_16bit<__nv_bfloat16>(a, error_flag, stream, launches, why);
   return launch_16bit<__half>(a, error_flag, stream, launches, why);
 }
