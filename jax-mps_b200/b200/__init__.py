@@ -622,13 +622,13 @@ class Client:
         place: row i goes to position slots[i] % page_size of page slots[i] // page_size (`slots`: whole numbers on the host; a
         negative one leaves its row out). Enqueued in the order of the client's work; slots are distinct."""
         index = _indices(slots, 1)
-        _check(_lib.b200_cache_write_pages(self._h, cache._h, rows._h, index.ctypes.data, len(index)))
+        _check(_lib.b200_cache_write_pages(self._h, cache._h, rows._h, index.tobytes(), len(index)))
 
     def copy_pages(self, cache: Buffer, pairs):
         """Page pairs[i][0] of a cache onto page pairs[i][1], keys and values of all layers, in place. Every source is read as it
         was before the call; destinations are distinct."""
         index = _indices(pairs, 2)
-        _check(_lib.b200_cache_copy_pages(self._h, cache._h, index.ctypes.data, len(index)))
+        _check(_lib.b200_cache_copy_pages(self._h, cache._h, index.tobytes(), len(index)))
 
     def close(self):
         if getattr(self, "_h", None) and self._owned:
