@@ -209,11 +209,6 @@ __device__ __forceinline__ uint32_t low_part(uint32_t v, uint32_t high) {
   const float rest = __uint_as_float(v) - __uint_as_float(high);
   return rest == rest ? high_part(__float_as_uint(rest)) : 0u;
 }
-__device__ __forceinline__ float power(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 __device__ __forceinline__ float column_max(float v) {             // over the lanes that hold the positions of a head
   v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 4));
   v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 8));

@@ -20,13 +20,6 @@ struct Sums {
 };
 constexpr float kLowest = -3.4028235e38f;
 
-// 2^v; denormal results are zero.
-__device__ __forceinline__ float power(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-
 // Maxima start at the type's lowest value, not at minus infinity, so that differences with them are numbers; a side that has no
 // weight at the joint maximum adds nothing, however far below it is.
 __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
@@ -44,6 +37,45 @@ __device__ __forceinline__ uint32_t order_of(float v) {
   if (v != v) return 0u;
   const uint32_t u = __float_as_uint(v + 0.f);
   return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+
+// The maximum and the sums of a block, in two steps: the maximum of all first, then everything in its units, so that joining is adding.
+// (With a maximum for each thread and sums joined as above, the joins of 4096 x 30522 in 32 bits were a quarter of all instructions.)
+template <int WARPS>
+__device__ __forceinline__ float block_max(float v, float (&shared)[WARPS]) {
+  v = warp_max(v);
+  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = shared[threadIdx.x % WARPS];
+#pragma unroll
+  for (int o = WARPS / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  return v;
+}
+template <int WARPS>
+__device__ __forceinline__ void block_sums(float& s, float& u, float2 (&shared)[WARPS]) {
+  s = warp_sum(s);
+  u = warp_sum(u);
+  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = make_float2(s, u);
+  __syncthreads();
+  s = shared[threadIdx.x % WARPS].x;
+  u = shared[threadIdx.x % WARPS].y;
+#pragma unroll
+  for (int o = WARPS / 2; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    u += __shfl_xor_sync(0xFFFFFFFFu, u, o);
+  }
+}
+// Two logits' share of the sums. The product of no weight and minus infinity is nothing, which the bound sees to; a NaN stays one.
+__device__ __forceinline__ void add_weights(uint64_t x, uint64_t minus_max, uint64_t& s, uint64_t& u) {
+  const uint64_t y = mul2(add2(x, minus_max), two(kLog2e, kLog2e)), e = two(power(first(y)), power(second(y)));
+  s = add2(s, e);
+  u = fma2(e, two(fmaxf(first(y), -200.f), fmaxf(second(y), -200.f)), u);
+}
+// p_j (c - d_entropy (x_j - n + entropy)) of two logits: d = x_j - n' with n = n' + rest, `scaled` -rest log2(e), `minus_dh` -d_entropy,
+// `others` c - d_entropy (entropy - rest).
+__device__ __forceinline__ uint64_t two_gradients(uint64_t d, uint64_t scaled, uint64_t minus_dh, uint64_t others) {
+  const uint64_t y = fma2(d, two(kLog2e, kLog2e), scaled);
+  return mul2(two(power(first(y)), power(second(y))), fma2(two(fmaxf(first(d), -200.f), fmaxf(second(d), -200.f)), minus_dh, others));
 }
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kHeld = 32;      // logits that a thread holds
@@ -164,7 +196,8 @@ template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads) probs_kernel(const __grid_constant__ Rows a) {
   pdl_prologue();
   constexpr int N = Pack<T>::N, NV = kHeld / N;
-  __shared__ Sums shared[kWarps];
+  __shared__ float maxima[kWarps];
+  __shared__ float2 sums[kWarps];
   __shared__ TopShared top;
   const int tid = threadIdx.x, seg = (int)(blockIdx.x % a.segments);
   const long long row = blockIdx.x / a.segments;
@@ -187,19 +220,16 @@ __global__ void __launch_bounds__(kThreads) probs_kernel(const __grid_constant__
   }
   Sums v = {kLowest, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) v.m = fmaxf(v.m, f[i]);
+  for (int i = 0; i < kHeld; i += 2) v.m = max3(v.m, f[i], f[i + 1]);
+  v.m = block_max(v.m, maxima);
+  uint64_t s[2] = {0, 0}, u[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    const float t = (f[i] - v.m) * kLog2e, e = power(t);
-    v.s += e;
-    v.u = fmaf(e, fmaxf(t, -200.f), v.u);                             // the product of no weight and minus infinity is nothing
-  }
-  v = warp_join(v);
-  if ((tid & 31) == 0) shared[tid >> 5] = v;
-  __syncthreads();
-  v = shared[0];
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) v = join(v, shared[w]);
+  for (int i = 0; i < kHeld; i += 2) add_weights(two(f[i], f[i + 1]), two(-v.m, -v.m), s[i / 2 % 2], u[i / 2 % 2]);
+  s[0] = add2(s[0], s[1]);
+  u[0] = add2(u[0], u[1]);
+  v.s = first(s[0]) + second(s[0]);
+  v.u = first(u[0]) + second(u[0]);
+  block_sums(v.s, v.u, sums);
   const bool whole = a.segments == 1;
   if (tid == 0) {
     if (whole) finish_row<T>(a, row, v);
@@ -275,10 +305,7 @@ __global__ void __launch_bounds__(kThreads) probs_grad_kernel(const __grid_const
   const int t = a.tokens[row];
   const float n = a.normalizer[row], low = a.remainder[row], h = a.entropy[row], dh = a.d_entropy[row], dl = t >= 0 && t < a.vocab ? a.d_log_prob[row] : 0.f;
   const float c = a.d_normalizer[row] - dl;
-  auto value = [&](float v, int j) {
-    const float y = (v - n) - low, p = power(y * kLog2e);
-    return (j == t ? dl : 0.f) + p * (c - dh * (fmaxf(y, -200.f) + h));
-  };
+  const uint64_t minus_n = two(-n, -n), scaled = two(-low * kLog2e, -low * kLog2e), minus_dh = two(-dh, -dh), others = two(c - dh * (h - low), c - dh * (h - low));
   uint4 held[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -295,11 +322,22 @@ __global__ void __launch_bounds__(kThreads) probs_grad_kernel(const __grid_const
       uint4 out;
       T* o = reinterpret_cast<T*>(&out);
 #pragma unroll
-      for (int e = 0; e < N; ++e) o[e] = from_float<T>(value(f[e], j + e));
+      for (int e = 0; e < N; e += 2) {
+        const uint64_t d = two_gradients(add2(two(f[e], f[e + 1]), minus_n), scaled, minus_dh, others);
+        f[e] = first(d);
+        f[e + 1] = second(d);
+      }
+      if ((unsigned)t - (unsigned)j < N) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] += j + e == t ? dl : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] = from_float<T>(f[e]);
       *(uint4*)(dx + j) = out;
     } else {
       for (int e = 0; e < N; ++e)
-        if (j + e >= 0 && j + e < a.vocab) dx[j + e] = from_float<T>(value(to_float(x[j + e]), j + e));
+        if (j + e >= 0 && j + e < a.vocab)
+          dx[j + e] = from_float<T>(first(two_gradients(add2(two(to_float(x[j + e]), 0.f), minus_n), scaled, minus_dh, others)) + (j + e == t ? dl : 0.f));
     }
   }
 }
@@ -307,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) probs_grad_kernel(const __grid_const
 // Both at once where the cotangents do not depend on the results: a block has a whole row in its registers, eight pieces of 16 bytes a
 // thread, takes the sums of it and writes the gradient, while the next row is on its way to shared memory, each thread's pieces to its
 // own place, so that no thread waits for another's. Bound by memory: the logits are read once and the gradient is written (4096 x 30522
-// in 32 bits 264 us by the two kernels above, 198 so, 153 at the rate of a copy).
+// in 32 bits 264 us by the two kernels above, 197 so, 153 at the rate of a copy; in bf16 178 and 76).
 constexpr int kRowThreads = 1024, kRowPieces = 8;
 
 struct Both {
@@ -323,11 +361,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) probs_both_kernel(const __grid
   pdl_prologue();
   constexpr int N = Pack<T>::N, W = kRowThreads / 32;
   extern __shared__ __align__(16) uint8_t ahead[];
-  __shared__ Sums shared[2][W];
+  __shared__ float maxima[W];
+  __shared__ float2 sums[W];
   const int tid = threadIdx.x, vocab = a.rows.vocab;
   const uint32_t mine = smem_u32(ahead) + tid * 16;
   auto offset = [&](const T* x) { return (int)(((unsigned long long)x / sizeof(T)) % N); };
-  auto inside = [&](int j) { return j >= 0 && j + N <= vocab; };
+  auto inside = [&](int j) { return (unsigned)j <= (unsigned)(vocab - N); };
+  // 16-bit data: pieces at a row's ends, which hold logits of its neighbours as well, are fetched whole and what is not the row's goes, but
+  // for those at the ends of the logits themselves. (Read one by one, 4096 x 30522 in bf16 267 us instead of 178; 32-bit data so 206 instead of 197.)
+  auto whole = [&](long long row, int j) {
+    return N == 4 ? inside(j) : j >= (row == 0 ? 0 : 1 - N) && j <= (row == a.rows.rows - 1 ? vocab - N : vocab - 1);
+  };
   auto fetch = [&](long long row) {
     if (row < a.rows.rows) {
       const T* x = (const T*)a.rows.x + row * vocab;
@@ -335,14 +379,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) probs_both_kernel(const __grid
 #pragma unroll
       for (int i = 0; i < kRowPieces; ++i) {
         const int j = (tid + i * kRowThreads) * N - off;
-        if (inside(j)) fetch16(mine + i * kRowThreads * 16, x + j);
+        if (whole(row, j)) fetch16(mine + i * kRowThreads * 16, x + j);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   fetch(blockIdx.x);
-  int turn = 0;
-  for (long long row = blockIdx.x; row < a.rows.rows; row += gridDim.x, turn ^= 1) {
+  for (long long row = blockIdx.x; row < a.rows.rows; row += gridDim.x) {
     const T* x = (const T*)a.rows.x + row * vocab;
     const int off = offset(x);
     const int t = a.rows.tokens[row];
@@ -357,8 +400,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) probs_both_kernel(const __grid
         held[i] = *(const uint4*)(ahead + (tid + i * kRowThreads) * 16);
       } else {
         T e[N];
+        const bool fetched = N == 8 && whole(row, j);
+        if (fetched) *reinterpret_cast<uint4*>(e) = *(const uint4*)(ahead + (tid + i * kRowThreads) * 16);
 #pragma unroll
-        for (int k = 0; k < N; ++k) e[k] = j + k >= 0 && j + k < vocab ? x[j + k] : from_float<T>(neg_inf());
+        for (int k = 0; k < N; ++k) {
+          if (j + k < 0 || j + k >= vocab) e[k] = from_float<T>(neg_inf());
+          else if (!fetched) e[k] = x[j + k];
+        }
         held[i] = *reinterpret_cast<const uint4*>(e);
       }
     }
@@ -366,26 +414,28 @@ __global__ void __launch_bounds__(kRowThreads, 1) probs_both_kernel(const __grid
     Sums v = {kLowest, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kRowPieces; ++i) {
+      if (N == 8 && i * kRowThreads * N >= vocab + off) break;        // (16-bit rows of up to 64 KB leave half of the pieces empty)
       float f[N];
       unpack<T>(held[i], f);
 #pragma unroll
-      for (int k = 0; k < N; ++k) v.m = fmaxf(v.m, f[k]);
+      for (int k = 0; k < N; k += 2) v.m = max3(v.m, f[k], f[k + 1]);
     }
+    v.m = block_max(v.m, maxima);                                     // (a barrier between any two uses of `maxima` and of `sums`)
+    const uint64_t minus_max = two(-v.m, -v.m);
+    uint64_t s[2] = {0, 0}, u[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < kRowPieces; ++i) {
+      if (N == 8 && i * kRowThreads * N >= vocab + off) break;
       float f[N];
       unpack<T>(held[i], f);
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const float y = (f[k] - v.m) * kLog2e, e = power(y);
-        v.s += e;
-        v.u = fmaf(e, fmaxf(y, -200.f), v.u);
-      }
+      for (int k = 0; k < N; k += 2) add_weights(two(f[k], f[k + 1]), minus_max, s[k / 2 % 2], u[k / 2 % 2]);
     }
-    v = warp_join(v);
-    if ((tid & 31) == 0) shared[turn][tid >> 5] = v;
-    __syncthreads();                                                  // (the other half of `shared` may still be read)
-    v = warp_join(shared[turn][tid & 31]);
+    s[0] = add2(s[0], s[1]);
+    u[0] = add2(u[0], u[1]);
+    v.s = first(s[0]) + second(s[0]);
+    v.u = first(u[0]) + second(u[0]);
+    block_sums(v.s, v.u, sums);
     const float ls = logf(v.s), n = v.s == 0.f ? neg_inf() : v.m + ls, low = (v.m - n) + ls, h = ls - v.u / v.s * kLn2;
     if (tid == 0) {
       a.rows.log_prob[row] = t >= 0 && t < vocab ? (at_token - v.m) - ls + (v.s == 0.f ? n - n : 0.f) : 0.f;
@@ -394,6 +444,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) probs_both_kernel(const __grid
       a.rows.remainder[row] = low;
     }
     const float c = dn - dl;
+    const uint64_t scaled = two(-ls * kLog2e, -ls * kLog2e), minus_dh = two(-dh, -dh), others = two(c - dh * (h - ls), c - dh * (h - ls));
     T* dx = (T*)a.grad.dx + row * vocab;
 #pragma unroll
     for (int i = 0; i < kRowPieces; ++i) {
@@ -404,10 +455,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) probs_both_kernel(const __grid
       uint4 out;
       T* o = reinterpret_cast<T*>(&out);
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const float y = (f[k] - n) - low, p = power(y * kLog2e);
-        o[k] = from_float<T>((j + k == t ? dl : 0.f) + p * (c - dh * (fmaxf(y, -200.f) + h)));
+      for (int k = 0; k < N; k += 2) {
+        const uint64_t d = two_gradients(add2(two(f[k], f[k + 1]), minus_max), scaled, minus_dh, others);
+        f[k] = first(d);
+        f[k + 1] = second(d);
       }
+      if ((unsigned)t - (unsigned)j < N) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) f[k] += j + k == t ? dl : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < N; ++k) o[k] = from_float<T>(f[k]);
       if (inside(j)) {
         __stcs((uint4*)(dx + j), out);
       } else {

@@ -29,12 +29,6 @@ __device__ __forceinline__ int length_of(const Prompt& a, int b) {
   return a.lengths ? min(max(a.lengths[b], 0), a.tokens) : a.tokens;
 }
 
-__device__ __forceinline__ float power(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-
 // Whether a position is seen; the keys' and values' sums run over these.
 __device__ __forceinline__ bool sees(const Prompt& a, int row, int key) {
   return key <= row && (a.window == 0 || row - key < a.window || key < a.sinks);
@@ -429,27 +423,6 @@ __device__ __forceinline__ uint32_t pair16(float lo, float hi) {
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-// Two floats in a register pair, for the instructions that take both at once.
-__device__ __forceinline__ uint64_t two(uint32_t x, uint32_t y) { return (uint64_t)y << 32 | x; }
-__device__ __forceinline__ uint64_t two(float x, float y) { return two(__float_as_uint(x), __float_as_uint(y)); }
-__device__ __forceinline__ float first(uint64_t v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float second(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 // What a block does next: its tiles of queries and the tiles of keys that they visit, those of the sinks in front of the window, then
 // the window's.
 template <int ITEMS>
