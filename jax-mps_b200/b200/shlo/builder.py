@@ -850,7 +850,8 @@ class Builder:
     def window_attention(self, q: Val, k: Val, v: Val, lengths: Val | None = None, *, scale: float | None = None, window: int = 0,
                          sinks: int = 0) -> Val:
         """Causal attention of whole prompts: q [batch, tokens, heads, head_dim], k and v [batch, tokens, kv_heads, head_dim], and for
-        a padded batch `lengths` i32[batch]; rows from a sequence's length on are zero and nobody sees them. `window`, `sinks` and
+        a padded batch `lengths` i32[batch]; rows from a sequence's length on are zero and nobody sees them, nor does what a row does not see
+        reach it, NaN and infinities included. `window`, `sinks` and
         `scale` as in paged_attention. No gradient."""
         xs = [q, k, v] + ([lengths] if lengths is not None else [])
         config = {"scale": None if scale is None else float(scale), "window": window, "sinks": sinks}

@@ -55,8 +55,8 @@ __device__ __forceinline__ int places(const Paged& a, const Span& s) { return ma
 
 // The rows of all sequences, one behind another, are cut into as many equal parts as there are blocks for a group of heads, whatever
 // the sequences' lengths: a block starts in the middle of one sequence and ends in the middle of another, and no block has more to
-// read than the others. (With parts that end with their sequence, 32 sequences of 0 to 4096 positions took 2.4 waves of blocks, 59 us;
-// 46 so.) Lengths are on the device only, so each block adds them up for itself.
+// read than the others. (With parts that end with their sequence, 32 sequences of 0 to 4096 positions took 2.4 waves of blocks:
+// 66 us instead of 55.) Lengths are on the device only, so each block adds them up for itself.
 template <int THREADS>
 struct Cut {
   int len;                            // places of a part

@@ -94,7 +94,8 @@ __device__ __noinline__ void mend_rows(const Prompt& a, int b, int h, int q0, in
 // lo + lo hi, hi a word rounded to the 19 bits that they read and lo what that leaves, rounded likewise; a tile's outputs are added up apart
 // and then to the others in 32 bits, since the tensor core cuts its sums. The order of the features within a step of 16 and of the keys
 // within a step of 8 is chosen so that fragments are loaded 16 bytes a thread, free of bank conflicts, and so that the scores' fragments
-// are the weights'.
+// are the weights'. Bound by the conversions and products, and for few queries by their chain: three prompts of up to 501 tokens, 12 heads of
+// 64, window 200 took 76 us on the FMA pipe, 38 with four warps of 16 queries each, 30 with two warps for the same queries.
 constexpr int kWideThreads = 128;
 template <int DP>
 struct Wide {
@@ -282,7 +283,7 @@ __global__ void __launch_bounds__(kWideThreads, Wide<DP>::PER_SM) prompt_wide_ke
     l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
     l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
   }
-  if (C::HALVES == 2 && tiles) {                                     // the second half's outputs to the first: a lane's own words, 16 warps' apart
+  if (C::HALVES == 2 && tiles) {                                     // the second half's outputs to the first: a lane's words, 32 apart
     float* at = stages + warp / 2 * (16 * (DP + 2)) + lane;
     if (half) {
 #pragma unroll
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(kWideThreads, Wide<DP>::PER_SM) prompt_wide_ke
 // first half of a row's weights is multiplied while the second is made. The outputs are scaled to a new maximum only when it has
 // grown by more than 2^8 since the last time; the weights are at most 2^8 until then, which no type minds, and the sums are divided
 // in the end by a sum that was taken in the same units.
-// Two prompts of 4096, 32 heads of 128, window 1024: one tile a block, two blocks an SM 206 us, two tiles a block 185 (652 TFLOP/s); with
+// Two prompts of 4096, 32 heads of 128, window 1024: one tile a block, two blocks an SM 206 us, two tiles a block 185 to 195 (650 TFLOP/s); with
 // two threads a row there too 192, with a quarter of the exponentials as polynomials on the FMA pipe 190. The chain of a tile - scores,
 // maximum, exponentials, outputs, 4300 cycles of which the tensor core works 2050 for both tiles - is what is left.
 // Products of a block run in the order in which its one thread issued them, so that scores may go where the weights of a product in
