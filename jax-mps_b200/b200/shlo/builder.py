@@ -833,6 +833,14 @@ class Builder:
         text = ", ".join(f"{k} = {v:.9e} : f32" if isinstance(v, float) else f"{k} = {int(v)} : i64" for k, v in config.items() if v is not None)
         return list(self.custom_call(f"b200.{name}", xs, result_types, attrs={"api_version": "4 : i32", "backend_config": "{" + text + "}"}))
 
+    def _no_gradient(self, what: str, outs: Sequence[Val], xs: Sequence[Val]):
+        """A cotangent of `outs` that would have to go on to `xs` is an error, not silently nothing."""
+        def vjp(_):
+            if not all(isinstance(x, _Stopped) for x in xs):
+                raise NotImplementedError(f"{what} has no gradient (stop_gradient its operands)")
+            return [None] * len(xs)
+        self.record(list(outs), list(xs), vjp)
+
     def paged_attention(self, q: Val, cache: Val, table: Val, lengths: Val, new: Val | None = None, *, layer: int = 0,
                         scale: float | None = None, window: int = 0, sinks: int = 0) -> Val:
         """Attention of one new token per sequence over a cache of pages: q [batch, heads, head_dim], `cache` [layers, 2 (keys,
@@ -845,7 +853,9 @@ class Builder:
         that the table names outside the cache are left out. f32, bf16 or f16, sums in 32 bits. No gradient."""
         xs = [q, cache, table, lengths] + ([new] if new is not None else [])
         config = {"layer": layer, "scale": None if scale is None else float(scale), "window": window, "sinks": sinks}
-        return self._operator("paged_attention", xs, [(q.shape, q.dtype)], config)[0]
+        out = self._operator("paged_attention", xs, [(q.shape, q.dtype)], config)
+        self._no_gradient("paged_attention", out, xs)
+        return out[0]
 
     def window_attention(self, q: Val, k: Val, v: Val, lengths: Val | None = None, *, scale: float | None = None, window: int = 0,
                          sinks: int = 0) -> Val:
@@ -855,7 +865,9 @@ class Builder:
         `scale` as in paged_attention. No gradient."""
         xs = [q, k, v] + ([lengths] if lengths is not None else [])
         config = {"scale": None if scale is None else float(scale), "window": window, "sinks": sinks}
-        return self._operator("window_attention", xs, [(q.shape, q.dtype)], config)[0]
+        out = self._operator("window_attention", xs, [(q.shape, q.dtype)], config)
+        self._no_gradient("window_attention", out, xs)
+        return out[0]
 
     def token_log_probs(self, logits: Val, tokens: Val, top: int = 0) -> list[Val]:
         """For logits [rows, vocab] (f32, bf16, f16) and tokens i32[rows]: the tokens' log probabilities (0 for a token outside the
@@ -870,6 +882,8 @@ class Builder:
         def vjp(g):
             return [self._operator("token_log_probs_grad", [logits, tokens, norm, rest, entropy, *g], [(logits.shape, logits.dtype)], {})[0], None]
         self.record([log_prob, entropy, norm], [logits, tokens], vjp)
+        if best:
+            self._no_gradient("the alternatives of token_log_probs", best[:1], [logits])
         return [log_prob, entropy, norm, *best]
 
     def optimization_barrier(self, xs: Sequence[Val]) -> list[Val]:

@@ -234,3 +234,21 @@ def test_scales_that_are_no_numbers(value):
     assert "scale = 5.000000000e-01 : f32" in text
     with pytest.raises(b200.B200Error, match="scale"):
         b200.compile_to_plan(text.replace("5.000000000e-01 : f32", value))
+
+
+def test_what_has_no_gradient_says_so():
+    b = Builder()
+    q, k = b.arg((1, 4, 2, 64), "f32"), b.arg((1, 4, 2, 64), "f32")
+    loss = b.reduce_sum(b.window_attention(b.mul(q, q), k, k), (0, 1, 2, 3))
+    with pytest.raises(NotImplementedError, match="window_attention"):
+        b.grad(loss, [q])
+    b = Builder()
+    x, t = b.arg((5, 100), "f32"), b.arg((5,), "i32")
+    values = b.token_log_probs(x, t, top=2)[3]
+    with pytest.raises(NotImplementedError, match="alternatives"):
+        b.grad(b.reduce_sum(values, (0, 1)), [x])
+    b = Builder()
+    x, y = b.arg((1, 4, 2, 64), "f32"), b.arg((1, 4, 2, 64), "f32")
+    s = b.stop_gradient(x)
+    loss = b.reduce_sum(b.mul(y, b.window_attention(s, s, s)), (0, 1, 2, 3))
+    assert b.grad(loss, [y])[0].shape == y.shape
