@@ -17,7 +17,9 @@
 namespace b200 {
 namespace {
 
-constexpr int kMinPart = 128;         // positions: a shorter part is not worth a place in the second pass
+// Positions: a shorter part is not worth a place in the second pass, and a shorter sequence is counted as so many, for what it costs a block
+// is mostly its own chain of loads (46 sequences of up to 10 positions in one block's row took 89 us, 5.5 in blocks of their own).
+constexpr int kMinPart = 128;
 
 struct Paged {
   const void *q, *cache, *fresh;
@@ -25,7 +27,7 @@ struct Paged {
   void* out;
   float* parts;                       // two places per block: for each query head dim outputs, the maximum and the sum
   int2* spans;                        // per sequence: its first part and how many it has
-  int batch, heads, kv_heads, dim, group, chunks, blocks, pages, page, width, window, sinks, has_new;
+  int batch, heads, kv_heads, dim, group, chunks, blocks, step, pages, page, width, window, sinks, has_new;
   unsigned page_inverse;              // 2^32 / page, cut
   long long plane;                    // elements between the keys and the values of a layer
   float scale;                        // of the scores, times log2(e)
@@ -50,8 +52,8 @@ __device__ __forceinline__ Span span_of(const Paged& a, int b) {
   s.seen = n - s.start + s.sinks;
   return s;
 }
-// Places of a row; one at least, so that every sequence has a block that writes its result.
-__device__ __forceinline__ int places(const Paged& a, const Span& s) { return max(1, s.seen + a.has_new); }
+// Places that a row counts as; every sequence has a block that writes its result.
+__device__ __forceinline__ int places(const Paged& a, const Span& s) { return max(kMinPart, s.seen + a.has_new); }
 
 // The rows of all sequences, one behind another, are cut into as many equal parts as there are blocks for a group of heads, whatever
 // the sequences' lengths: a block starts in the middle of one sequence and ends in the middle of another, and no block has more to
@@ -88,7 +90,7 @@ __device__ __forceinline__ bool cut_of(const Paged& a, int block, Cut<THREADS>& 
     total += sums[w];
   }
   r.total = total;
-  r.len = (int)min(max((long long)kMinPart, ((total + a.blocks - 1) / a.blocks + 15) / 16 * 16), 1LL << 30);
+  r.len = (int)min(max((long long)kMinPart, ((total + a.blocks - 1) / a.blocks + a.step - 1) / a.step * a.step), 1LL << 30);
   const long long want = (long long)block * r.len;
   if (want >= total) return false;
   long long at = upto - mine;
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NT>::WARPS * 32, Ring<T, DP, NT>::
   for (long long at = cut.at; cut.b < a.batch && at < to0; ++cut.b) {
     const int b = cut.b;
     const Span span = span_of(a, b);
-    const int n = places(a, span), from = (int)(max(from0, at) - at), end = (int)min((long long)n, to0 - at);
+    const int n = places(a, span), from = (int)(max(from0, at) - at), end = (int)min((long long)(span.seen + a.has_new), to0 - at);
     const int first = (int)(at / cut.len), count = (int)((at + n - 1) / cut.len) - first + 1;      // the blocks that share the sequence
     at += n;
 
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NT>::WARPS * 32, Ring<T, DP, NT>::
           q[k][t][i] = h < nh && d < D ? *(const uint32_t*)(src + d) : 0u;
         }
     }
-    const int ntiles = (end - from + 15) / 16;
+    const int ntiles = end > from ? (end - from + 15) / 16 : 0;
     const uint8_t *keys = (const uint8_t*)a.cache, *fresh_key = (const uint8_t*)a.fresh + ((long long)b * a.kv_heads + kvh) * D * (long long)sizeof(T);
     const long long plane = a.plane * (long long)sizeof(T), fresh_plane = (long long)a.batch * a.kv_heads * D * (long long)sizeof(T);
     // lanes look up a position each (the upper half those of the lower once more), in front of the tile that asks for them
@@ -618,6 +620,7 @@ auto with_ring(const OperatorLaunch& op, F&& f) {
 
 struct Shape {
   int chunks, blocks;                 // groups of heads; blocks for each
+  int step;                           // of a part's length
   bool several;                       // whether a sequence can have several parts
 };
 Shape shape_of(const OperatorLaunch& op) {
@@ -629,9 +632,10 @@ Shape shape_of(const OperatorLaunch& op) {
     // places that the tables have room for
     long long cap = (long long)op.width * op.page;
     if (op.window > 0) cap = std::min<long long>(cap, (long long)op.window + op.sinks);
-    cap = std::max<long long>(1, cap + op.has_new);
+    cap = std::max<long long>(kMinPart, cap + op.has_new);
     s.blocks = (int)std::min<long long>(std::max(1, kSMs * R::PER_SM / s.chunks), (cap * op.batch + kMinPart - 1) / kMinPart);
-    s.several = cap * op.batch > kMinPart && cap > 1;
+    s.several = cap > kMinPart;
+    s.step = s.several ? 16 : kMinPart;                             // sequences of one part each stay whole
     return s;
   });
 }
@@ -644,7 +648,7 @@ const char* paged_attention_plan(OperatorLaunch& op) {
   if ((long long)op.width * op.page >= (1LL << 30)) return "tables of 2^30 positions and more";
   if ((long long)op.pages * op.page * op.kv_heads * op.dim * (op.type == 0 ? 4 : 2) >= 16 * 0xFFFFFFFELL) return "64 GB and more of a layer's keys";
   const Shape s = shape_of(op);
-  if (((long long)op.width * op.page + 1) * op.batch / s.blocks >= (1LL << 30)) return "more positions than the blocks can share";
+  if (((long long)op.width * op.page + kMinPart) * op.batch / s.blocks >= (1LL << 30) - kMinPart) return "more positions than the blocks can share";
   if ((long long)s.blocks * s.chunks >= (1LL << 31) || (long long)op.batch * op.heads >= (1LL << 31)) return "too many sequences and heads";
   op.scratch_bytes = spans_bytes(op) + (s.several ? 2LL * s.blocks * op.heads * (op.dim + 4) * 4 : 0);
   op.launches = s.several ? 2 : 1;
@@ -669,6 +673,7 @@ cudaError_t launch_paged_attention(const OperatorLaunch& op, void* const* args, 
   const Shape s = shape_of(op);
   a.chunks = s.chunks;
   a.blocks = s.blocks;
+  a.step = s.step;
   return with_ring(op, [&](auto t, auto dp, auto nt) -> cudaError_t {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value, NT = decltype(nt)::value;

@@ -105,6 +105,15 @@ def test_paged_attention_many_sequences(client):
     check_paged(client, *paged_case(rng, rng.integers(0, 40, 1500).tolist(), 2, 1, 8, 4, "bf16", True), "bf16")
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("lens", [[0] * 5, [1] * 300, [127, 0, 126, 1] * 9, [128, 0, 5] * 40, [3] * 700 + [400]])
+def test_paged_attention_short_sequences(client, dt, lens):
+    """Sequences that are one part each, and some beside a longer one; the token beside the cache makes 128 of 127."""
+    for new in (False, True):
+        rng = np.random.default_rng(len(lens) + new)
+        check_paged(client, *paged_case(rng, lens, 4, 2, 64, 16, dt, new), dt)
+
+
 def test_paged_attention_layer_scale_and_shared_pages(client):
     rng = np.random.default_rng(11)
     q, cache, table, lengths, fresh = paged_case(rng, [30, 45, 45], 4, 2, 64, 16, "bf16", True, layers=3)
@@ -551,6 +560,38 @@ def test_operators_in_a_recorded_program_and_a_loop(client):
             got = [o.to_numpy() for o in exe.execute([client.buffer_from_host(v) for v in args])]
             for g, w in zip(got, want):
                 np.testing.assert_allclose(g, w, rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_prompts_and_losses_in_a_recorded_program(client, dt):
+    """Kernels that read arguments through tensor maps and a loss with its gradient, replayed with other buffers each time."""
+    b = Builder()
+    q, k, v = (b.arg((2, 150, h, 64), dt) for h in (4, 2, 2))
+    n, x, t, w = b.arg((2,), "i32"), b.arg((296, 8200), dt), b.arg((296,), "i32"), b.arg((296,), "f32")
+    outs, y = [], q
+    for window in (0, 100, 33, 1):
+        y = b.window_attention(y, k, v, n, window=window, sinks=2 if window else 0)
+        outs.append(b.mul(y, b.full(y.shape, 2.0, dt)))
+    lp = b.token_log_probs(x, t)[0]
+    outs += [lp, *b.grad(b.reduce_sum(b.mul(lp, w), (0,)), [x])]
+    exe = client.compile(b.module(outs))
+    for seed in range(3):
+        rng = np.random.default_rng(seed)
+        arrays = [rounded(rng.standard_normal(s), dt) for s in ((2, 150, 4, 64), (2, 150, 2, 64), (2, 150, 2, 64))]
+        lengths, logits = np.array([150 - seed, 77 + seed], np.int32), rounded(rng.standard_normal((296, 8200)), dt)
+        tokens, weights = rng.integers(0, 8200, 296).astype(np.int32), rng.standard_normal(296).astype(np.float32)
+        for _ in range(2):
+            bufs = [put(client, a, dt) for a in arrays] + [client.buffer_from_host(lengths), put(client, logits, dt), client.buffer_from_host(tokens), client.buffer_from_host(weights)]
+            got = [np.asarray(o.to_numpy(), np.float64) for o in exe.execute(bufs)]
+            q = arrays[0]
+            for i, window in enumerate((0, 100, 33, 1)):
+                want, mag, top = operators.window_attention(q, *arrays[1:], lengths, window=window, sinks=2 if window else 0, bounds=True)
+                assert (np.abs(got[i] / 2 - want) <= attention_tolerance(want, mag, top, 150, 64, dt, 0.0 if dt == "f32" else U[dt])).all()
+                q = got[i] / 2                             # exact: what the next call read
+            # a log probability: differences of numbers below 16 rounded a few times, and a sum of 8200 terms that are good to 2^-22
+            assert (np.abs(got[4] - operators.token_log_probs(logits, tokens)[0]) <= 8 * 16 * E + 2.0 ** -21).all()
+            want = operators.token_log_probs_grad(logits, tokens, weights, np.zeros(296), np.zeros(296))
+            assert (np.abs(got[5] - want) <= U[dt] * np.abs(want) + 2.0 ** -18 * np.abs(weights)[:, None]).all()
 
 
 def test_two_calls_in_flight(client):
