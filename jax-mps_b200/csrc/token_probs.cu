@@ -345,7 +345,8 @@ __global__ void __launch_bounds__(kThreads) probs_grad_kernel(const __grid_const
 // Both at once where the cotangents do not depend on the results: a block has a whole row in its registers, eight pieces of 16 bytes a
 // thread, takes the sums of it and writes the gradient, while the next row is on its way to shared memory, each thread's pieces to its
 // own place, so that no thread waits for another's. Bound by memory: the logits are read once and the gradient is written (4096 x 30522
-// in 32 bits 264 us by the two kernels above, 197 so, 153 at the rate of a copy; in bf16 178 and 76).
+// in 32 bits 264 us by the two kernels above, 191 to 197 so, 153 at the rate of a copy; in bf16 128 and 76; 8141 x 8446 in 32 bits 130
+// and 84). Blocks of 1024 threads for all rows, of which an SM has room for one, took 178 and 236 us for the last two.
 constexpr int kRowThreads = 1024, kRowPieces = 8;
 
 struct Both {
@@ -356,10 +357,10 @@ __device__ __forceinline__ void fetch16(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads, 1) probs_both_kernel(const __grid_constant__ Both a) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, kRowThreads / THREADS) probs_both_kernel(const __grid_constant__ Both a) {
   pdl_prologue();
-  constexpr int N = Pack<T>::N, W = kRowThreads / 32;
+  constexpr int N = Pack<T>::N, W = THREADS / 32;
   extern __shared__ __align__(16) uint8_t ahead[];
   __shared__ float maxima[W];
   __shared__ float2 sums[W];
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) probs_both_kernel(const __grid
   auto offset = [&](const T* x) { return (int)(((unsigned long long)x / sizeof(T)) % N); };
   auto inside = [&](int j) { return (unsigned)j <= (unsigned)(vocab - N); };
   // 16-bit data: pieces at a row's ends, which hold logits of its neighbours as well, are fetched whole and what is not the row's goes, but
-  // for those at the ends of the logits themselves. (Read one by one, 4096 x 30522 in bf16 267 us instead of 178; 32-bit data so 206 instead of 197.)
+  // for those at the ends of the logits themselves. (Read one by one, 4096 x 30522 in bf16 267 us instead of 178, with 1024 threads a block; 32-bit data so 206 instead of 197.)
   auto whole = [&](long long row, int j) {
     return N == 4 ? inside(j) : j >= (row == 0 ? 0 : 1 - N) && j <= (row == a.rows.rows - 1 ? vocab - N : vocab - 1);
   };
@@ -378,8 +379,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) probs_both_kernel(const __grid
       const int off = offset(x);
 #pragma unroll
       for (int i = 0; i < kRowPieces; ++i) {
-        const int j = (tid + i * kRowThreads) * N - off;
-        if (whole(row, j)) fetch16(mine + i * kRowThreads * 16, x + j);
+        const int j = (tid + i * THREADS) * N - off;
+        if (whole(row, j)) fetch16(mine + i * THREADS * 16, x + j);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -395,13 +396,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) probs_both_kernel(const __grid
     asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < kRowPieces; ++i) {
-      const int j = (tid + i * kRowThreads) * N - off;
+      const int j = (tid + i * THREADS) * N - off;
       if (inside(j)) {
-        held[i] = *(const uint4*)(ahead + (tid + i * kRowThreads) * 16);
+        held[i] = *(const uint4*)(ahead + (tid + i * THREADS) * 16);
       } else {
         T e[N];
         const bool fetched = N == 8 && whole(row, j);
-        if (fetched) *reinterpret_cast<uint4*>(e) = *(const uint4*)(ahead + (tid + i * kRowThreads) * 16);
+        if (fetched) *reinterpret_cast<uint4*>(e) = *(const uint4*)(ahead + (tid + i * THREADS) * 16);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
           if (j + k < 0 || j + k >= vocab) e[k] = from_float<T>(neg_inf());
@@ -414,7 +415,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) probs_both_kernel(const __grid
     Sums v = {kLowest, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kRowPieces; ++i) {
-      if (N == 8 && i * kRowThreads * N >= vocab + off) break;        // (16-bit rows of up to 64 KB leave half of the pieces empty)
+      if (N == 8 && i * THREADS * N >= vocab + off) break;        // (rows leave up to half of the pieces empty)
       float f[N];
       unpack<T>(held[i], f);
 #pragma unroll
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) probs_both_kernel(const __grid
     uint64_t s[2] = {0, 0}, u[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < kRowPieces; ++i) {
-      if (N == 8 && i * kRowThreads * N >= vocab + off) break;
+      if (N == 8 && i * THREADS * N >= vocab + off) break;
       float f[N];
       unpack<T>(held[i], f);
 #pragma unroll
@@ -448,7 +449,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) probs_both_kernel(const __grid
     T* dx = (T*)a.grad.dx + row * vocab;
 #pragma unroll
     for (int i = 0; i < kRowPieces; ++i) {
-      const int j = (tid + i * kRowThreads) * N - off;
+      const int j = (tid + i * THREADS) * N - off;
       if (j >= vocab) break;
       float f[N];
       unpack<T>(held[i], f);
@@ -501,12 +502,23 @@ cudaError_t launch_grad(const Grad& a, long long rows, cudaStream_t stream, int*
   return launch_op(probs_grad_kernel<T>, dim3((unsigned)(rows * a.segments)), kThreads, 0, stream, launches, a);
 }
 
-template <typename T>
+long long row_bytes(const OperatorLaunch& op) { return (long long)op.vocab * (op.type == 0 ? 4 : 2) + 32; }      // with what its ends may share
+
+template <typename T, int THREADS>
 cudaError_t launch_both(const Both& a, cudaStream_t stream, int* launches) {
   static bool done[64] = {};
-  constexpr size_t smem = (size_t)kRowThreads * kRowPieces * 16;
-  if (cudaError_t e = allow_smem(probs_both_kernel<T>, smem, done)) return e;
-  return launch_op(probs_both_kernel<T>, dim3((unsigned)std::min<long long>(a.rows.rows, kSMs)), kRowThreads, smem, stream, launches, a);
+  constexpr size_t smem = (size_t)THREADS * kRowPieces * 16;
+  if (cudaError_t e = allow_smem(probs_both_kernel<T, THREADS>, smem, done)) return e;
+  const dim3 grid((unsigned)std::min<long long>(a.rows.rows, kSMs * (kRowThreads / THREADS)));
+  return launch_op(probs_both_kernel<T, THREADS>, grid, THREADS, smem, stream, launches, a);
+}
+template <typename T>
+cudaError_t launch_both(const OperatorLaunch& op, const Both& a, cudaStream_t stream, int* launches) {
+  // the smallest blocks that hold a row: the more of them an SM has, the more of a row's waits another's arithmetic fills
+  const long long bytes = row_bytes(op), each = kRowPieces * 16;
+  if (bytes <= 256 * each) return launch_both<T, 256>(a, stream, launches);
+  if (bytes <= 512 * each) return launch_both<T, 512>(a, stream, launches);
+  return launch_both<T, kRowThreads>(a, stream, launches);
 }
 
 Rows rows_of(const OperatorLaunch& op, void* const* results, void* const* operands) {
@@ -526,8 +538,8 @@ Rows rows_of(const OperatorLaunch& op, void* const* results, void* const* operan
 
 // Rows that a block's registers hold and that give each thread something, and enough of them for every SM to have two.
 bool token_log_probs_at_once(const OperatorLaunch& op) {
-  const long long bytes = (long long)op.vocab * (op.type == 0 ? 4 : 2);
-  return op.top == 0 && op.rows >= 2 * kSMs && bytes >= kRowThreads * 16 && bytes + 32 <= kRowThreads * kRowPieces * 16LL;
+  const long long bytes = row_bytes(op);
+  return op.top == 0 && op.rows >= 2 * kSMs && bytes - 32 >= kRowThreads * 16 && bytes <= kRowThreads * kRowPieces * 16LL;
 }
 
 const char* token_log_probs_plan(OperatorLaunch& op) {
@@ -583,9 +595,9 @@ cudaError_t launch_token_log_probs_both(const OperatorLaunch& op, void* const* a
   a.grad.d_log_prob = (const float*)args[7];
   a.grad.d_entropy = (const float*)args[8];
   a.grad.d_normalizer = (const float*)args[9];
-  if (op.type == 0) return launch_both<float>(a, stream, launches);
-  if (op.type == 1) return launch_both<__nv_bfloat16>(a, stream, launches);
-  return launch_both<__half>(a, stream, launches);
+  if (op.type == 0) return launch_both<float>(op, a, stream, launches);
+  if (op.type == 1) return launch_both<__nv_bfloat16>(op, a, stream, launches);
+  return launch_both<__half>(op, a, stream, launches);
 }
 
 }  // namespace b200
