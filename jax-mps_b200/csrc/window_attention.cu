@@ -88,22 +88,22 @@ __device__ __noinline__ void mend_rows(const Prompt& a, int b, int h, int q0, in
 }
 
 // ---- 32-bit data ---------------------------------------------------------------------------------------
-// A block takes 64 queries of a head, a warp 16 of them, and goes through 32 places of its row of keys at a time: first the sinks that lie
+// A block takes 32 or 64 queries of a head, a warp 16 of them, and goes through 32 places of its row of keys at a time: first the sinks that lie
 // in front of its first query's window, then from that window's first key on, whichever key that is, so that no tile is half empty. Keys
 // and values come by cp.async, a tile ahead. Both products run on the tensor cores by mma.sync (tf32 m16n8k8) in three parts, hi hi + hi
 // lo + lo hi, hi a word rounded to the 19 bits that they read and lo what that leaves, rounded likewise; a tile's outputs are added up apart
 // and then to the others in 32 bits, since the tensor core cuts its sums. The order of the features within a step of 16 and of the keys
 // within a step of 8 is chosen so that fragments are loaded 16 bytes a thread, free of bank conflicts, and so that the scores' fragments
 // are the weights'. Bound by the conversions and products, and for few queries by their chain: three prompts of up to 501 tokens, 12 heads of
-// 64, window 200 took 76 us on the FMA pipe, 38 with four warps of 16 queries each, 30 with two warps for the same queries.
-constexpr int kWideThreads = 128;
+// 64, window 200 took 76 us on the FMA pipe, 38 with four warps of 16 queries each, 30 with two warps for the same queries. Three of up to 1356, 2
+// heads of 72: 195 us with four warps, 128 with eight, two for the same queries; 256 features leave no room for a second half of a tile.
 template <int DP>
 struct Wide {
   // warps that share their queries, each with its own 32 keys of a tile: two where the tiles leave room for it
-  static constexpr int HALVES = DP == 64 ? 2 : 1, ROWS = 64 / HALVES, KEYS = 32 * HALVES;
+  static constexpr int HALVES = DP <= 128 ? 2 : 1, THREADS = DP == 128 ? 256 : 128, ROWS = THREADS / 2 / HALVES, KEYS = 32 * HALVES;
   static constexpr int KP = DP + 16, VP = DP + 4;                    // floats between rows of queries and keys, of values
   static constexpr int STAGE = KEYS * (KP + VP), SMEM = (ROWS * KP + 2 * STAGE) * 4;
-  static constexpr int PER_SM = DP <= 128 ? 2 : 1;
+  static constexpr int PER_SM = DP == 64 ? 2 : 1;
   static constexpr bool HELD = DP == 64;                             // the queries' parts stay in registers
   static_assert(HALVES == 1 || ROWS * (DP + 2) <= STAGE, "no room for the halves' outputs");
   static_assert((SMEM + 1024) * PER_SM <= 233472, "more than an SM has");
@@ -131,7 +131,7 @@ __device__ __forceinline__ void mma_four(float (&c)[4][4], const uint32_t (&hi)[
 }
 
 template <int DP>
-__global__ void __launch_bounds__(kWideThreads, Wide<DP>::PER_SM) prompt_wide_kernel(const __grid_constant__ Prompt a) {
+__global__ void __launch_bounds__(Wide<DP>::THREADS, Wide<DP>::PER_SM) prompt_wide_kernel(const __grid_constant__ Prompt a) {
   pdl_prologue();
   using C = Wide<DP>;
   constexpr int P = DP / 4, KEYS = C::KEYS;
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kWideThreads, Wide<DP>::PER_SM) prompt_wide_ke
     if (tile < tiles) {
       float *ks = stages + (tile & 1) * C::STAGE + r0 * C::KP + c0, *vs = stages + (tile & 1) * C::STAGE + KEYS * C::KP + r0 * C::VP + c0;
 #pragma unroll 8
-      for (int r = 0; r < KEYS; r += kWideThreads / P) {
+      for (int r = 0; r < KEYS; r += C::THREADS / P) {
         const int place = tile * KEYS + r0 + r;
         const bool there = place < places && c0 < D;
         const long long at = there ? base + (place + (place < sinks ? 0 : shift)) * stride : 0;
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kWideThreads, Wide<DP>::PER_SM) prompt_wide_ke
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   if (tiles) {
-    for (int r = r0; r < C::ROWS; r += kWideThreads / P) {
+    for (int r = r0; r < C::ROWS; r += C::THREADS / P) {
       const bool there = q0 + r < n && c0 < D;
       copy(qs + r * C::KP + c0, (const float*)a.q + (there ? (((long long)b * a.tokens + q0 + r) * a.heads + h) * D + c0 : 0), there);
     }
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kWideThreads, Wide<DP>::PER_SM) prompt_wide_ke
       }
   }
   // (with all rows that are not finite: parts of infinities are no numbers)
-  if (__syncthreads_or(odd != odd)) mend_rows<float>(a, b, h, q0, C::ROWS, warp, kWideThreads / 32, true);
+  if (__syncthreads_or(odd != odd)) mend_rows<float>(a, b, h, q0, C::ROWS, warp, C::THREADS / 32, true);
 }
 
 // ---- 16-bit data on the tensor cores -------------------------------------------------------------------
@@ -813,7 +813,7 @@ template <int DP>
 cudaError_t launch_wide(const Prompt& a, cudaStream_t stream, int* launches) {
   static bool done[64] = {};
   if (cudaError_t e = allow_smem(prompt_wide_kernel<DP>, Wide<DP>::SMEM, done)) return e;
-  return launch_op(prompt_wide_kernel<DP>, dim3((unsigned)((a.tokens + Wide<DP>::ROWS - 1) / Wide<DP>::ROWS), (unsigned)a.heads, (unsigned)a.batch), kWideThreads,
+  return launch_op(prompt_wide_kernel<DP>, dim3((unsigned)((a.tokens + Wide<DP>::ROWS - 1) / Wide<DP>::ROWS), (unsigned)a.heads, (unsigned)a.batch), Wide<DP>::THREADS,
                    Wide<DP>::SMEM, stream, launches, a);
 }
 
