@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) probs_grad_kernel(const __grid_const
 // Both at once where the cotangents do not depend on the results: a block has a whole row in its registers, eight pieces of 16 bytes a
 // thread, takes the sums of it and writes the gradient, while the next row is on its way to shared memory, each thread's pieces to its
 // own place, so that no thread waits for another's. Bound by memory: the logits are read once and the gradient is written (4096 x 30522
-// in 32 bits 264 us by the two kernels above, 191 to 197 so, 153 at the rate of a copy; in bf16 128 and 76; 8141 x 8446 in 32 bits 130
+// in 32 bits 264 us by the two kernels above, 190 to 201 so, 153 at the rate of a copy; in bf16 128 and 76; 8141 x 8446 in 32 bits 130
 // and 84). Blocks of 1024 threads for all rows, of which an SM has room for one, took 178 and 236 us for the last two.
 constexpr int kRowThreads = 1024, kRowPieces = 8;
 
