@@ -458,8 +458,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t *qs = smem, *ks = qs + ITEMS * C::TILE, *vs = ks + S * C::TILE;
   uint64_t* bars = (uint64_t*)(vs + S * C::TILE);
-  // queries are there, are done with; keys and values likewise, a stage each; scores of a place; weights of a place, two halves; outputs
-  // of a tile have all products so far, have been read; both threads of a row have spoken; nothing is under way
+  // queries are there, are done with; keys and values likewise, a stage each; scores of a place; weights of a place, two halves, the first
+  // with the outputs scaled; outputs of a tile have all products so far, have been read; both threads of a row have spoken; nothing is
+  // under way
   constexpr int Q_FULL = 0, Q_EMPTY = 1, K_FULL = 2, K_EMPTY = K_FULL + S, V_FULL = K_EMPTY + S, V_EMPTY = V_FULL + S, S_FULL = V_EMPTY + S, P_FULL = S_FULL + 2,
                 PV_DONE = P_FULL + 4, O_EMPTY = PV_DONE + 2, AGREED = O_EMPTY + 2, DRAINED = AGREED + 4, BARRIERS = DRAINED + 1;
   static_assert(BARRIERS * 8 + 12 <= 512, "barriers");
@@ -470,8 +471,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid
   uint8_t* stage = (uint8_t*)(said + 4 * kRows);                     // [warp][row][32 results]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, D = a.dim;
   if (tid == 0) {
+    // (with two threads a row, the first half's weights are announced by its four warps, and by the four others that the outputs are scaled)
     for (int k = 0; k < BARRIERS; ++k)
-      mbar_init(bar(k), k >= P_FULL && k < PV_DONE ? 4 : k >= O_EMPTY && k < AGREED ? 8 / ITEMS : k >= AGREED && k < DRAINED ? 2 : 1);
+      mbar_init(bar(k), k >= P_FULL && k < PV_DONE ? (ITEMS == 1 && (k - P_FULL) % 2 == 0 ? 8 : 4) : k >= O_EMPTY && k < AGREED ? 8 / ITEMS : k >= AGREED && k < DRAINED ? 2 : 1);
     *failed = 0;
     *strange = 0;                                                    // whether a result is not finite
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -703,6 +705,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid
 #pragma unroll 1
             for (int c = half * (DP / 2); c < (ITEMS == 2 ? DP : (half + 1) * (DP / 2)); c += 8) scale8(outputs(u) + mine + c, keep);
           }
+        }
+        if (ITEMS == 1 && half) {
+          // a product adds to all columns of the outputs, so the first one waits for what this thread has scaled of them too, not only for
+          // the weights of the other
+          stored();
+          before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(P_FULL + 2 * place(u, j)));
         }
         const float ref = m == neg_inf() ? 0.f : m * a.scale - shift;
         const uint64_t minus = two(-ref, -ref);

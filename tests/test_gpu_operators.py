@@ -605,3 +605,38 @@ def test_two_calls_in_flight(client):
     outs = [exe.execute(bufs[i % 2])[0] for i in range(10)]
     for i, o in enumerate(outs):
         np.testing.assert_allclose(o.to_numpy(), operators.paged_attention(*cases[i % 2][:4]), rtol=1e-4, atol=1e-5)
+
+
+# ---- maxima that grow from tile to tile ---------------------------------------------------------------------
+def rising_case(rng, B, T, H, KH, D, dt, growth):
+    """Scores that rise by `growth` (of the logarithm to base 2) from each 128 keys to the next, and values that fall by as much, so that every
+    tile is as large a share of the result as the last, although all but it are scaled down on the way there."""
+    q, k, v = prompt_case(rng, B, T, H, KH, D, dt)
+    tile = np.arange(T) // 128
+    q[..., 0], q[..., 1:] = 1.0, q[..., 1:] / 16
+    k[..., 0] = (tile * (growth * np.log(2)))[None, :, None]
+    k[..., 1:] /= 16
+    most = 13 if dt == "f16" else growth * (T // 128) // 2
+    v = v * 2.0 ** (most - tile * float(growth))[None, :, None, None]
+    return [rounded(x, dt) for x in (q, k, v)]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("B,H,KH,D", [(1, 2, 1, 64), (1, 1, 1, 72), (2, 2, 2, 128), (1, 2, 1, 192), (1, 2, 1, 256), (19, 8, 4, 64), (19, 8, 8, 128)])
+@pytest.mark.parametrize("growth,window,sinks", [(9, 0, 0), (9, 300, 3), (5, 0, 0)])
+def test_window_attention_of_rising_scores(client, dt, B, H, KH, D, growth, window, sinks):
+    """One tile of queries a block (with two threads a row), two tiles of one head (19 x 8 heads, 2 tiles each), two heads: in each the outputs are
+    scaled down, not to nothing, at every tile or every other one."""
+    T = 250 if B > 1 and H == 8 else 384 if dt == "f16" else 700
+    rng = np.random.default_rng(D + growth)
+    q, k, v = rising_case(rng, B, T, H, KH, D, dt, growth)
+    arrays, dts = [q, k, v], [dt] * 3
+    kw = dict(window=window, sinks=sinks, scale=1.0)
+    first, second = (run(client, lambda b, q, k, v: b.window_attention(q, k, v, **kw), arrays, dts)[0] for _ in range(2))
+    np.testing.assert_array_equal(first, second)
+    some = sorted({0, B - 1})
+    want, mag, top = operators.window_attention(q[some], k[some], v[some], bounds=True, **kw)
+    # (weights are in units of a maximum that is at most 2^8 below their tile's: none is small enough to lose bits beside its own rounding)
+    tol = attention_tolerance(want, mag, top, T, D, dt, 0.0 if dt == "f32" else U[dt])
+    bad = ~(np.abs(first[some] - want) <= tol)
+    assert not bad.any(), (float(np.abs(first[some] - want)[bad].max()), np.argwhere(bad)[:5].tolist(), int(bad.sum()))
