@@ -1284,7 +1284,8 @@ struct DecodeAttentionFusion {
 
 // A loss and its gradient: b200.token_log_probs and the b200.token_log_probs_grad of the same logits become one operation that reads the
 // logits once, where the rows fit (token_log_probs_at_once) and the cotangents do not depend on the log probabilities. What the
-// cotangents are made of moves in front of it.
+// cotangents are made of moves in front of it. Calls that do not have the types and attributes of the two stay as they are and are
+// refused as such.
 // ---------------------------------------------------------------------------
 void join_loss_and_gradient(Block* b) {
   for (auto& op : b->ops)
@@ -1299,6 +1300,14 @@ void join_loss_and_gradient(Block* b) {
       continue;
     const TensorType& x = probs->operands[0]->type;
     if (x.rank() != 2 || (x.dt != DT::F32 && x.dt != DT::BF16 && x.dt != DT::F16) || x.dims[1] >= (1LL << 30)) continue;
+    bool fits = grad->attrs.empty() && grad->results[0]->type == x;
+    for (auto& kv : probs->attrs) fits = fits && kv.first == "top" && strtod(kv.second.c_str(), nullptr) == 0.0;
+    TensorType row;
+    row.dt = DT::F32;
+    row.dims = {x.dims[0]};
+    for (Value* v : probs->results) fits = fits && v->type == row;
+    for (int k = 5; k < 8; k++) fits = fits && grad->operands[k]->type == row;
+    if (!fits) continue;
     OperatorLaunch o;
     o.type = x.dt == DT::F32 ? 0 : 1;
     o.rows = x.dims[0];
@@ -3027,7 +3036,8 @@ struct Planner {
       const bool grad = op->name == "b200.token_log_probs_grad", both = op->name == "b200.token_log_probs_both";
       o.kind = grad ? OperatorLaunch::TOKEN_LOG_PROBS_GRAD : both ? OperatorLaunch::TOKEN_LOG_PROBS_BOTH : OperatorLaunch::TOKEN_LOG_PROBS;
       o.top = grad ? 0 : (int)whole("top", 0, 0, 128);
-      if (!both) count(grad ? 8 : 2, grad ? 8 : 2, grad ? 1 : o.top ? 6 : 4);
+      const size_t takes = grad ? 8 : both ? 5 : 2;
+      count(takes, takes, grad ? 1 : both ? 5 : o.top ? 6 : 4);
       o.type = type_of(in[0], "the logits");
       rank(in[0], "the logits", 2);
       o.rows = in[0]->type.dims[0];
@@ -3037,6 +3047,8 @@ struct Planner {
       want(in[1], "the tokens", DT::I32, {o.rows});
       if (both) {
         for (int k = 2; k < 5; k++) want(in[k], "a cotangent", DT::F32, {o.rows});
+        for (int k = 0; k < 4; k++) want(out[k], "a result", DT::F32, {o.rows});
+        want(out[4], "the result", in[0]->type.dt, in[0]->type.dims);
       } else if (grad) {
         for (int k = 2; k < 8; k++) want(in[k], "an operand of the gradient", DT::F32, {o.rows});
         want(out[0], "the result", in[0]->type.dt, in[0]->type.dims);

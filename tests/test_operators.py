@@ -252,3 +252,30 @@ def test_what_has_no_gradient_says_so():
     s = b.stop_gradient(x)
     loss = b.reduce_sum(b.mul(y, b.window_attention(s, s, s)), (0, 1, 2, 3))
     assert b.grad(loss, [y])[0].shape == y.shape
+
+
+def joined_text(R=300, V=5000, dt="f32", probs=None, grad=None, config="", top=""):
+    """A loss and its gradient as the assembly writes them, `probs` and `grad` the types that they claim to give."""
+    x, r = f"tensor<{R}x{V}x{dt}>", f"tensor<{R}xf32>"
+    probs, grad = [f"tensor<{t}>" for t in probs or [f"{R}xf32"] * 4], f"tensor<{grad or f'{R}x{V}x{dt}'}>"
+    return f"""module @jit_f {{
+  func.func public @main(%x: {x}, %t: tensor<{R}xi32>, %g: {r}) -> ({probs[0]}, {grad}) {{
+    %p:4 = "stablehlo.custom_call"(%x, %t) <{{call_target_name = "b200.token_log_probs", backend_config = {{{top}}}}}> : ({x}, tensor<{R}xi32>) -> ({", ".join(probs)})
+    %d = "stablehlo.custom_call"(%x, %t, %p#2, %p#3, %p#1, %g, %g, %g) <{{call_target_name = "b200.token_log_probs_grad", backend_config = {{{config}}}}}> : ({x}, tensor<{R}xi32>, {probs[2]}, {probs[3]}, {probs[1]}, {r}, {r}, {r}) -> {grad}
+    "func.return"(%p#0, %d) : ({probs[0]}, {grad}) -> ()
+  }}
+}}"""
+
+
+@pytest.mark.parametrize("R,joined", [(300, True), (200, False)])
+@pytest.mark.parametrize("kw,why", [
+    (dict(grad="2x2xbf16"), "result"), (dict(grad="{R}x5000xbf16"), "result"), (dict(grad="{R}x4999xf32"), "result"), (dict(probs=["3xf32"] + ["{R}xf32"] * 3), "result"),
+    (dict(probs=["{R}xf32"] * 3 + ["{R}xf64"]), "result"), (dict(config="top = 0 : i64"), "no attribute"), (dict(config="scale = 1.0 : f32"), "no attribute"),
+    (dict(top="top = 3 : i64"), "results"), (dict(top="scale = 1.0 : f32"), "no attribute")])
+def test_a_loss_with_its_gradient_refuses_what_either_would(R, joined, kw, why):
+    """Also in rows that both are made of by one kernel, which writes results of the sizes that the logits give."""
+    plan, _ = b200.compile_to_plan(joined_text(R))
+    assert ("token_log_probs_both" in plan) == joined
+    kw = {k: [t.format(R=R) for t in v] if isinstance(v, list) else v.format(R=R) for k, v in kw.items()}
+    with pytest.raises(b200.B200Error, match=why):
+        b200.compile_to_plan(joined_text(R, **kw))
