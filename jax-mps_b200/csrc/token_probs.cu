@@ -256,7 +256,9 @@ template <typename T>
 __device__ __forceinline__ Sums row_sums(const Rows& a, long long row) {
   Sums v = {kLowest, 0.f, 0.f};
   for (int i = threadIdx.x & 31; i < a.segments; i += 32) v = join(v, a.sums[row * a.segments + i]);
-  return warp_join(v);
+  v = warp_join(v);
+  // the first lane's for all: the last bit depends on which of two was joined to which, and no alternative's on the thread that has it
+  return {__shfl_sync(0xFFFFFFFFu, v.m, 0), __shfl_sync(0xFFFFFFFFu, v.s, 0), __shfl_sync(0xFFFFFFFFu, v.u, 0)};
 }
 template <typename T>
 __global__ void __launch_bounds__(kThreads) probs_join_kernel(const __grid_constant__ Rows a) {

@@ -640,3 +640,23 @@ def test_window_attention_of_rising_scores(client, dt, B, H, KH, D, growth, wind
     tol = attention_tolerance(want, mag, top, T, D, dt, 0.0 if dt == "f32" else U[dt])
     bad = ~(np.abs(first[some] - want) <= tol)
     assert not bad.any(), (float(np.abs(first[some] - want)[bad].max()), np.argwhere(bad)[:5].tolist(), int(bad.sum()))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("R,V,top", [(1, 256000, 64), (3, 128257, 128), (40, 30522, 20)])
+def test_alternatives_repeat_themselves(client, dt, R, V, top):
+    """Rows of several parts: whichever thread finds an alternative, its log probability has the same bits, in each call and for equal logits."""
+    rng = np.random.default_rng(V)
+    x = rounded(rng.standard_normal((R, V)) * 4, dt)
+    x[:, 1::2] = x[:, :V // 2 * 2:2]                                     # equal logits among the best
+    b = Builder()
+    a, t = b.arg(x.shape, dt), b.arg((R,), "i32")
+    exe = client.compile(b.module(b.token_log_probs(a, t, top=top)))
+    bufs = [put(client, x, dt), client.buffer_from_host(np.zeros(R, np.int32))]
+    first = [o.to_numpy() for o in exe.execute(bufs)]
+    for r in range(R):
+        best = x[r, first[4][r]]
+        assert (np.diff(first[3][r])[np.diff(best) == 0] == 0).all()
+    for _ in range(20):
+        for g, w in zip(exe.execute(bufs), first):
+            np.testing.assert_array_equal(g.to_numpy(), w)
