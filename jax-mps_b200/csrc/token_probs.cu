@@ -480,10 +480,13 @@ __global__ void __launch_bounds__(THREADS, kRowThreads / THREADS) probs_both_ker
   }
 }
 
+constexpr int kJoined = 64 * kThreads;                        // alternatives of a row's segments that the block that joins them holds
+
 // Segments of a row: as few as hold it (a first piece that starts in front of the row counts), and more for few rows, down to 2048
-// logits, so that the blocks fill the chip.
+// logits, so that the blocks fill the chip, as long as their alternatives can be joined.
 int segments_of(const OperatorLaunch& op) {
-  const long long least = (op.vocab + 8 + kSegment - 1) / kSegment, most = std::max<long long>(least, op.vocab / 2048);
+  const long long least = ((long long)op.vocab + 8 + kSegment - 1) / kSegment;
+  const long long most = std::max<long long>(least, std::min<long long>(op.vocab / 2048, op.top ? kJoined / op.top : op.vocab));
   return (int)std::max<long long>(least, std::min<long long>(most, 2 * kSMs / std::max<long long>(1, op.rows)));
 }
 
@@ -552,7 +555,7 @@ const char* token_log_probs_plan(OperatorLaunch& op) {
   }
   const bool grad = op.kind == OperatorLaunch::TOKEN_LOG_PROBS_GRAD;
   int s = segments_of(op);
-  if (op.top && (long long)s * op.top > 64 * kThreads) return "more alternatives than this vocabulary's segments leave room for";
+  if (op.top && (long long)s * op.top > kJoined) return "more alternatives than this vocabulary's segments leave room for";
   if (op.rows * s >= (1LL << 31)) return "too many logits";
   const bool several = !grad && s > 1;
   op.scratch_bytes = several ? op.rows * s * (12 + 8LL * op.top) + 16 : 0;

@@ -660,3 +660,10 @@ def test_alternatives_repeat_themselves(client, dt, R, V, top):
     for _ in range(20):
         for g, w in zip(exe.execute(bufs), first):
             np.testing.assert_array_equal(g.to_numpy(), w)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("R,V,top", [(1, 300000, 128), (2, 300000, 100), (1, 600001, 64)])
+def test_alternatives_of_few_rows_of_large_vocabularies(client, dt, R, V, top):
+    rng = np.random.default_rng(V + R)
+    check_probs(client, rounded(rng.standard_normal((R, V)) * 4, dt), rng.integers(0, V, R), top, dt)

@@ -279,3 +279,21 @@ def test_a_loss_with_its_gradient_refuses_what_either_would(R, joined, kw, why):
     kw = {k: [t.format(R=R) for t in v] if isinstance(v, list) else v.format(R=R) for k, v in kw.items()}
     with pytest.raises(b200.B200Error, match=why):
         b200.compile_to_plan(joined_text(R, **kw))
+
+
+@pytest.mark.parametrize("R", [1, 2, 3, 8, 300])
+@pytest.mark.parametrize("V,top", [(300000, 128), (600000, 64), (1000000, 128), (2000000, 64)])
+def test_alternatives_of_few_rows_of_large_vocabularies(R, V, top):
+    """What is taken of many rows is taken of one: few rows are cut into more parts only as far as their alternatives can be joined."""
+    b = Builder()
+    x, t = b.arg((R, V), "bf16"), b.arg((R,), "i32")
+    plan, _ = b200.compile_to_plan(b.module(b.token_log_probs(x, t, top=top)))
+    assert "operator token_log_probs top" in plan
+
+
+@pytest.mark.parametrize("R", [1, 300])
+def test_more_alternatives_than_can_be_joined(R):
+    b = Builder()
+    x, t = b.arg((R, 1200000), "bf16"), b.arg((R,), "i32")
+    with pytest.raises(b200.B200Error, match="more alternatives"):
+        b200.compile_to_plan(b.module(b.token_log_probs(x, t, top=128)))
