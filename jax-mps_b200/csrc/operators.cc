@@ -6,17 +6,6 @@ namespace b200 {
 bool operators_programmatic_launch = true;
 void set_operators_programmatic_launch(bool on) { operators_programmatic_launch = on; }
 
-const char* operator_name(const OperatorLaunch& op) {
-  switch (op.kind) {
-    case OperatorLaunch::PAGED_ATTENTION: return "b200.paged_attention";
-    case OperatorLaunch::WINDOW_ATTENTION: return "b200.window_attention";
-    case OperatorLaunch::TOKEN_LOG_PROBS: return "b200.token_log_probs";
-    case OperatorLaunch::TOKEN_LOG_PROBS_GRAD: return "b200.token_log_probs_grad";
-    case OperatorLaunch::TOKEN_LOG_PROBS_BOTH: return "b200.token_log_probs_both";
-    default: return "none";
-  }
-}
-
 const char* operator_plan(OperatorLaunch& op) {
   switch (op.kind) {
     case OperatorLaunch::PAGED_ATTENTION: return paged_attention_plan(op);

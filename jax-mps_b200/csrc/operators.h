@@ -27,7 +27,6 @@ struct OperatorLaunch {
 
 // Chooses kernels and sizes the scratch memory; null, or why the operator cannot run.
 const char* operator_plan(OperatorLaunch& op);
-const char* operator_name(const OperatorLaunch& op);
 void set_operators_programmatic_launch(bool on);
 // `args`: results, then operands, in the order of the custom call.
 cudaError_t launch_operator(const OperatorLaunch& op, void* const* args, void* scratch, int* error_flag, cudaStream_t stream, int* launches, const char** why);
