@@ -461,6 +461,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NT>::WARPS * 32, Ring<T, DP, NT>::
       for (int s = 0; s < AHEAD; ++s) there[s] = there[s + 1];
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    bool odd[NT][2], any_odd = false;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -468,8 +469,83 @@ __global__ void __launch_bounds__(Ring<T, DP, NT>::WARPS * 32, Ring<T, DP, NT>::
         l[t][i] += __shfl_xor_sync(0xFFFFFFFFu, l[t][i], 4);
         l[t][i] += __shfl_xor_sync(0xFFFFFFFFu, l[t][i], 8);
         l[t][i] += __shfl_xor_sync(0xFFFFFFFFu, l[t][i], 16);
-        if (lane < 4) { stats[warp][t * 8 + lane * 2 + i][0] = m[t][i]; stats[warp][t * 8 + lane * 2 + i][1] = l[t][i]; }
+        // Products in parts make no numbers of infinities: a part of a weight may be zero or below it, and one of an infinite word is no
+        // number. (16-bit scores are products in one part, so that weights without a number are what the definition gives.)
+        bool nan = false;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) nan |= o[k][t][i] != o[k][t][i] || o[k][t][2 + i] != o[k][t][2 + i];
+        nan = (nan && (WIDE || l[t][i] == l[t][i])) || (WIDE && l[t][i] != l[t][i]);
+        odd[t][i] = (__ballot_sync(0xFFFFFFFFu, nan) & 0x11111111u << (lane & 3)) && t * 8 + lane % 4 * 2 + i < nh;
+        any_odd |= odd[t][i];
       }
+    if (__any_sync(0xFFFFFFFFu, any_odd)) {
+      // Such heads are made again from the warp's positions, one after another with whole words and weights, in the places of the products'
+      // fragments. Nothing is spent on it otherwise.
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (odd[t][i]) {
+            m[t][i] = neg_inf();
+            l[t][i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) o[k][t][i] = o[k][t][2 + i] = 0.f;
+          }
+#pragma unroll 1
+      for (int tile = warp; tile < ntiles; tile += W)
+#pragma unroll 1
+        for (int place = from + tile * 16; place < min(end, from + tile * 16 + 16); ++place) {
+          const unsigned where = key_at(a, look_up(a, span, b, place, end), kvh, row_pieces);
+          if (where == kNowhere) continue;
+          const uint8_t* row = where == kFresh ? fresh_key : keys + ((unsigned long long)where << 4);
+          const T *key = (const T*)row, *value = (const T*)(row + (where == kFresh ? fresh_plane : plane));
+          float x[NT][2] = {};
+#pragma unroll 1
+          for (int d = lane / 4; d < D; d += 8) {
+            const float kd = to_float(key[d]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int h = min(t * 8 + lane % 4 * 2 + i, nh - 1);
+                x[t][i] = fmaf(to_float(((const T*)a.q)[((long long)b * a.heads + h0 + h) * D + d]), kd, x[t][i]);
+              }
+          }
+          float keep[NT][2], p[NT][2];
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+              for (int by = 4; by < 32; by *= 2) x[t][i] += __shfl_xor_sync(0xFFFFFFFFu, x[t][i], by);
+              x[t][i] *= a.scale;
+              const float top = fmaxf(m[t][i], x[t][i]), ref = top == neg_inf() ? 0.f : top;
+              keep[t][i] = power(m[t][i] - ref);
+              p[t][i] = power(LIFT > 0.f ? x[t][i] - ref + LIFT : x[t][i] - ref);
+              if (odd[t][i]) {
+                m[t][i] = top;
+                l[t][i] = l[t][i] * keep[t][i] + p[t][i];
+              }
+            }
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int d = k * 16 + e * 8 + lane / 4;
+              const float v = d < D ? to_float(value[d]) : 0.f;
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                  if (odd[t][i]) o[k][t][2 * e + i] = fmaf(p[t][i], v, o[k][t][2 * e + i] * keep[t][i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (lane < 4) { stats[warp][t * 8 + lane * 2 + i][0] = m[t][i]; stats[warp][t * 8 + lane * 2 + i][1] = l[t][i]; }
     __syncthreads();                                                // nobody reads the ring any more, all maxima are known
     // the warps' outputs go through the ring's memory in units of the block's maximum: [warp][head][feature]
     float* os = reinterpret_cast<float*>(ring);

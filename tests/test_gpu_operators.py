@@ -667,3 +667,34 @@ def test_alternatives_repeat_themselves(client, dt, R, V, top):
 def test_alternatives_of_few_rows_of_large_vocabularies(client, dt, R, V, top):
     rng = np.random.default_rng(V + R)
     check_probs(client, rounded(rng.standard_normal((R, V)) * 4, dt), rng.integers(0, V, R), top, dt)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("H,KH,D,S", [(4, 1, 64, 16), (3, 3, 128, 7), (2, 1, 72, 8), (24, 1, 192, 16), (6, 2, 256, 5)])
+@pytest.mark.parametrize("lens", [[20, 3, 0], [3001, 400], [17] * 40 + [700]])
+def test_paged_attention_of_values_that_are_no_numbers(client, dt, H, KH, D, S, lens):
+    """Visible infinities and NaN in values and keys, the type's largest value, in the cache and beside it: what the definition makes of them, in
+    the features and heads that they reach and in no others."""
+    rng = np.random.default_rng(D + len(lens))
+    q, cache, table, lengths, fresh = paged_case(rng, lens, H, KH, D, S, dt, True)
+    values = cache[0, 1]
+
+    def at(b, j):
+        return table[b, j // S], j % S
+    values[at(0, 1)][:, 3], values[at(0, 2)][:, 3] = np.inf, np.inf
+    values[at(0, lens[0] - 1)][:, 5], values[at(0, 0)][:, D - 1] = -np.inf, np.nan
+    values[at(0, 4)][:, 10], values[at(0, 5)][:, 10] = np.inf, -np.inf
+    values[at(0, 6)][:, 11] = {"f32": 3.4028235e38, "bf16": 3.3895314e38, "f16": 65504.0}[dt]
+    fresh[1, 1, :, 7], fresh[1, -1, 0, 2] = np.inf, -np.inf
+    cache[0, 0][at(len(lens) - 2 if lens[-1] == 0 else len(lens) - 1, 1)][KH - 1, 9] = np.inf        # a score without a bound: to one side no weight, to the other no number
+    with np.errstate(all="ignore"):
+        got = run(client, lambda b, q, c, t, n, new: b.paged_attention(q, c, t, n, new=new), [q, cache, table, lengths, fresh], [dt, dt, "i32", "i32", dt])[0]
+        raw = operators.paged_attention(q, cache, table, lengths, fresh)
+        known = [np.where(np.isfinite(t), t, 0.0) for t in (cache, fresh)]
+        _, mag, top = operators.paged_attention(q, known[0], table, lengths, known[1], bounds=True)
+        tol = attention_tolerance(np.where(np.isfinite(raw), raw, 0.0), mag, top, max(lens) + 1, D, dt, 0.0 if dt == "f32" else U[dt] ** 2)
+        assert np.isinf(raw).any() and np.isnan(raw).any() and np.isfinite(raw).mean() > 0.3
+        np.testing.assert_array_equal(np.isnan(got), np.isnan(raw))
+        np.testing.assert_array_equal(got[np.isinf(raw)], raw[np.isinf(raw)])
+        fine = np.isfinite(raw)
+        assert (np.abs(got - raw)[fine] <= tol[fine]).all(), float((np.abs(got - raw) - tol)[fine].max())
