@@ -815,7 +815,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid
   for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
     const Unit<ITEMS> w(a, unit);
 #pragma unroll 1
-    for (int u = 0; u < ITEMS; ++u) mend_rows<T>(a, w.b, w.head[u], w.q0[u], kRows, warp, kMmaThreads / 32, false);
+    for (int u = 0; u < ITEMS; ++u)
+      // (f16: with all rows that are not finite, for weights that it has no number for are zero beside a visible infinity too)
+      mend_rows<T>(a, w.b, w.head[u], w.q0[u], kRows, warp, kMmaThreads / 32, std::is_same<T, __half>::value);
   }
 }
 

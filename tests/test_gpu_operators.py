@@ -698,3 +698,29 @@ def test_paged_attention_of_values_that_are_no_numbers(client, dt, H, KH, D, S, 
         np.testing.assert_array_equal(got[np.isinf(raw)], raw[np.isinf(raw)])
         fine = np.isfinite(raw)
         assert (np.abs(got - raw)[fine] <= tol[fine]).all(), float((np.abs(got - raw) - tol)[fine].max())
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("B,H,KH,D", [(1, 2, 1, 64), (1, 1, 1, 256), (19, 8, 4, 64), (19, 8, 8, 128)])
+def test_window_attention_of_infinities_with_little_weight(client, dt, B, H, KH, D):
+    """A visible infinity with e^-25 of the largest weight, which is no number of f16 any more, is an infinity all the same."""
+    T = 250
+    rng = np.random.default_rng(D)
+    q, k, v = prompt_case(rng, B, T, H, KH, D, dt)
+    q[..., 0], q[..., 1:] = 1.0, q[..., 1:] / 16
+    k[..., 0], k[..., 1:] = 0.0, k[..., 1:] / 16
+    k[:, 7, :, 0], k[:, 150, :, 0] = -25.0, -25.0
+    v[:, 7, :, 3], v[:, 150, :, 3], v[:, 150, :, 6] = np.inf, -np.inf, -np.inf
+    q, k, v = (rounded(x, dt) for x in (q, k, v))
+    got = run(client, lambda b, q, k, v: b.window_attention(q, k, v, scale=1.0), [q, k, v], [dt] * 3)[0]
+    some = sorted({0, B - 1})
+    with np.errstate(all="ignore"):
+        raw = operators.window_attention(q[some], k[some], v[some], scale=1.0)
+        want, mag, top = operators.window_attention(q[some], k[some], np.where(np.isfinite(v[some]), v[some], 0.0), scale=1.0, bounds=True)
+    got = got[some]
+    assert (raw[:, 7:150, :, 3] == np.inf).all() and np.isnan(raw[:, 150:, :, 3]).all() and (raw[:, 150:, :, 6] == -np.inf).all()
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(raw))
+    np.testing.assert_array_equal(got[np.isinf(raw)], raw[np.isinf(raw)])
+    fine = np.isfinite(raw)
+    tol = attention_tolerance(want, mag, top, T, D, dt, 0.0 if dt == "f32" else U[dt])
+    assert (np.abs(got - want)[fine] <= tol[fine]).all()
