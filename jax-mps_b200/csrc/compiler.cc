@@ -178,6 +178,31 @@ std::map<std::string, std::string> custom_call_config(const Op& op) {
   return out;
 }
 
+// The operators read and write row-major arrays: `operand_layouts` and `result_layouts` of a custom call, which list the dimensions of each from
+// the one whose elements lie side by side, have to say that where they stand.
+void check_layouts(const Op& op, const std::string& name) {
+  for (const char* key : {"operand_layouts", "result_layouts"}) {
+    if (!op.has(key)) continue;
+    const std::string& raw = op.attr(key);
+    const auto& values = key[0] == 'o' ? op.operands : op.results;
+    auto refuse = [&]() { throw CompileError(name + ": " + key + " has to be row-major for each of " + std::to_string(values.size()) + ", got " + raw); };
+    size_t n = 0;
+    for (size_t at = raw.find("dense<"); at != std::string::npos; at = raw.find("dense<", at), n++) {
+      at += 6;
+      const size_t end = raw.find('>', at);
+      if (end == std::string::npos || n >= values.size()) refuse();
+      int64_t next = (int64_t)values[n]->type.dims.size() - 1;
+      for (; at < end; at++) {
+        if (raw[at] < '0' || raw[at] > '9') continue;
+        if (strtoll(raw.c_str() + at, nullptr, 10) != next--) refuse();
+        while (at + 1 < end && raw[at + 1] >= '0' && raw[at + 1] <= '9') at++;
+      }
+      if (next != -1) refuse();
+    }
+    if (n != values.size()) refuse();
+  }
+}
+
 struct Inliner {
   Module& m;
   std::map<Value*, Value*> remap;
@@ -312,6 +337,7 @@ struct Inliner {
       // Operators of large language models: the operation by its own name, checked and lowered by Planner::lower_operator. Any
       // other target of this name space stays a custom_call and is refused as one.
       if (is_operator(tgt)) {
+        check_layouts(*op, tgt);
         auto config = custom_call_config(*op);
         op->name = tgt;
         op->attrs = std::move(config);

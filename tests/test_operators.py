@@ -297,3 +297,31 @@ def test_more_alternatives_than_can_be_joined(R):
     x, t = b.arg((R, 1200000), "bf16"), b.arg((R,), "i32")
     with pytest.raises(b200.B200Error, match="more alternatives"):
         b200.compile_to_plan(b.module(b.token_log_probs(x, t, top=128)))
+
+
+@pytest.mark.parametrize("generic", [False, True])
+@pytest.mark.parametrize("operands,results,fine", [
+    ("dense<[2, 1, 0]> : tensor<3xindex>, dense<[5, 4, 3, 2, 1, 0]> : tensor<6xindex>, dense<[1, 0]> : tensor<2xindex>, dense<0> : tensor<1xindex>", "dense<[2, 1, 0]> : tensor<3xindex>", True),
+    ("dense<[2, 1, 0]> : tensor<3xindex>, dense<[5, 4, 3, 2, 1, 0]> : tensor<6xindex>, dense<[0, 1]> : tensor<2xindex>, dense<0> : tensor<1xindex>", "dense<[2, 1, 0]> : tensor<3xindex>", False),
+    ("dense<[2, 1, 0]> : tensor<3xindex>, dense<[5, 4, 3, 2, 1, 0]> : tensor<6xindex>, dense<[1, 0]> : tensor<2xindex>, dense<0> : tensor<1xindex>", "dense<[1, 2, 0]> : tensor<3xindex>", False),
+    ("dense<[2, 1, 0]> : tensor<3xindex>, dense<[5, 4, 3, 2, 1, 0]> : tensor<6xindex>, dense<[1, 0]> : tensor<2xindex>", "dense<[2, 1, 0]> : tensor<3xindex>", False),
+    ("dense<[2, 1, 0]> : tensor<3xindex>, dense<[4, 5, 3, 2, 1, 0]> : tensor<6xindex>, dense<[1, 0]> : tensor<2xindex>, dense<0> : tensor<1xindex>", "dense<[2, 1, 0]> : tensor<3xindex>", False),
+    ("dense<[2, 1, 0]> : tensor<3xindex>, dense<[4, 3, 2, 1, 0]> : tensor<5xindex>, dense<[1, 0]> : tensor<2xindex>, dense<0> : tensor<1xindex>", "dense<[2, 1, 0]> : tensor<3xindex>", False),
+])
+def test_layouts_are_row_major(operands, results, fine, generic):
+    """jax.ffi.ffi_call writes a layout for each operand and result; any but row-major is refused, not read in the wrong order."""
+    types = ["tensor<1x2x8xf32>", "tensor<2x2x3x4x1x8xf32>", "tensor<1x2xi32>", "tensor<1xi32>"]
+    attrs = f"api_version = 4 : i32, operand_layouts = [{operands}], result_layouts = [{results}]"
+    call = (f'"stablehlo.custom_call"(%arg0, %arg1, %arg2, %arg3) <{{call_target_name = "b200.paged_attention", {attrs}}}>' if generic else
+            f"stablehlo.custom_call @b200.paged_attention(%arg0, %arg1, %arg2, %arg3) {{{attrs}}}")
+    text = f"""module @jit_f {{
+  func.func public @main({", ".join(f"%arg{i}: {t}" for i, t in enumerate(types))}) -> tensor<1x2x8xf32> {{
+    %0 = {call} : ({", ".join(types)}) -> tensor<1x2x8xf32>
+    return %0 : tensor<1x2x8xf32>
+  }}
+}}"""
+    if fine:
+        assert "operator paged_attention" in b200.compile_to_plan(text)[0]
+    else:
+        with pytest.raises(b200.B200Error, match="b200.paged_attention.*layout"):
+            b200.compile_to_plan(text)
