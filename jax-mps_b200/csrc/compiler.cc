@@ -148,15 +148,17 @@ bool is_operator(const std::string& name) {
 }
 
 // Attributes of a custom call: what stands in its `backend_config` (or `mhlo.backend_config`) dictionary.
-std::map<std::string, std::string> custom_call_config(const Op& op) {
+std::map<std::string, std::string> custom_call_config(const Op& op, const std::string& name) {
   std::map<std::string, std::string> out;
   for (const char* key : {"backend_config", "mhlo.backend_config"}) {
     if (!op.has(key)) continue;
     const std::string& raw = op.attr(key);
     size_t i = raw.find_first_not_of(" \t\n");
-    if (i == std::string::npos || raw[i] != '{') continue;               // the string form says nothing here
+    if (i == std::string::npos || raw.compare(i, std::string::npos, "\"\"") == 0) continue;
+    // attributes in a string (api_version 2 and before) would be taken for none
+    if (raw[i] != '{') throw CompileError(name + ": backend_config has to be a dictionary, got " + raw);
     const size_t end = raw.rfind('}');
-    if (end == std::string::npos || end < i) throw CompileError("custom_call: unreadable backend_config " + raw);
+    if (end == std::string::npos || end < i) throw CompileError(name + ": unreadable backend_config " + raw);
     i++;
     while (i < end) {
       size_t comma = raw.find(',', i);
@@ -169,7 +171,7 @@ std::map<std::string, std::string> custom_call_config(const Op& op) {
         return a == std::string::npos ? std::string() : s.substr(a, z - a + 1);
       };
       if (eq == std::string::npos) {
-        if (!trimmed(item).empty()) throw CompileError("custom_call: unreadable backend_config " + raw);
+        if (!trimmed(item).empty()) throw CompileError(name + ": unreadable backend_config " + raw);
         continue;
       }
       out[trimmed(item.substr(0, eq))] = trimmed(item.substr(eq + 1));
@@ -338,7 +340,7 @@ struct Inliner {
       // other target of this name space stays a custom_call and is refused as one.
       if (is_operator(tgt)) {
         check_layouts(*op, tgt);
-        auto config = custom_call_config(*op);
+        auto config = custom_call_config(*op, tgt);
         op->name = tgt;
         op->attrs = std::move(config);
         process(std::move(op), b);

@@ -1,4 +1,6 @@
 """Operators that programs name as custom calls, and the bookkeeping of the paged cache: what needs no GPU."""
+import re
+
 import numpy as np
 import pytest
 
@@ -325,3 +327,15 @@ def test_layouts_are_row_major(operands, results, fine, generic):
     else:
         with pytest.raises(b200.B200Error, match="b200.paged_attention.*layout"):
             b200.compile_to_plan(text)
+
+
+@pytest.mark.parametrize("config", ['"{window = 5 : i64}"', '"\\7B\\22window\\22: 5}"', '"window=5"'])
+def test_a_configuration_in_a_string_is_refused(config):
+    """Attributes that would not be read; a call of the earlier form without any is fine."""
+    text = paged_text(window=5)
+    given = re.sub(r"backend_config = \{[^}]*\}", lambda m: f"backend_config = {config}", text)
+    assert given != text
+    with pytest.raises(b200.B200Error, match="b200.paged_attention.*backend_config"):
+        b200.compile_to_plan(given)
+    plain = re.sub(r"backend_config = \{[^}]*\}", 'backend_config = ""', text).replace("api_version = 4", "api_version = 2")
+    assert "operator paged_attention" in b200.compile_to_plan(plain)[0]
