@@ -290,10 +290,21 @@ struct StatusWord {
 // (a bounded device-side wait ran out) when the two differ once the copies have landed. Executions follow one another on
 // the compute stream, so the counter behind one is the counter in front of the next: one copy per execution. Plans
 // whose kernels wait for nothing are not watched at all.
+// A buffer that several executions wrote (a cache) has one for each that is not known to have ended well, in a list that is not changed
+// once it has been made: events of reads hold it.
+struct ReadyEvent;
 struct ExecStatus {
   std::shared_ptr<StatusWord> before, after;
-  uint64_t first = 0, last = 0;         // numbers of the executions on their client, from the first to the last
-  bool failed() const { return before && after && *after->word != *before->word; }
+  std::shared_ptr<ExecStatus> also;     // of those that wrote earlier
+  std::shared_ptr<ReadyEvent> landed;   // in a list: behind the copies of both words
+  int length = 1, most = 0;             // in a list: how many, and from how many on those that ended well are taken out
+  bool watched() const { return before && after; }
+  bool gave_up() const { return watched() && *after->word != *before->word; }
+  bool failed() const {
+    for (const ExecStatus* s = this; s; s = s->also.get())
+      if (s->gave_up()) return true;
+    return false;
+  }
 };
 
 // An event from the client's pool, recorded once; all results of an execution share theirs.
@@ -409,7 +420,6 @@ struct b200_client {
   int* status_block = nullptr;          // pinned words handed to executions
   static constexpr int kStatusWords = 8192;
   std::shared_ptr<StatusWord> last_status;      // the counter behind the last watched execution; null: not known
-  uint64_t watched_executions = 0;
   // Small parts that executions and buffers hand back and forth: free status words and events (under a lock of their
   // own, taken by destructors on any thread).
   std::mutex parts_mu;
@@ -2555,7 +2565,6 @@ b200_error* b200_executable_execute(b200_executable* exe, b200_buffer* const* ar
   std::shared_ptr<ExecStatus> status;
   if (exe->lp->watched || c->armed_wait_polls > 0) {
     status = std::make_shared<ExecStatus>();
-    status->first = status->last = ++c->watched_executions;
     status->before = c->last_status;
     status->after = new_status_word(c);
     if (!status->before && (status->before = new_status_word(c)))
@@ -3087,18 +3096,35 @@ bool repeats(const int32_t* index, size_t n, size_t stride, int64_t limit) {
   return false;
 }
 
-// What is known of a buffer that two executions wrote: the counter from in front of the first to behind the last.
-std::shared_ptr<ExecStatus> both_statuses(const std::shared_ptr<ExecStatus>& a, const std::shared_ptr<ExecStatus>& b) {
-  auto watched = [](const std::shared_ptr<ExecStatus>& s) { return s && s->before && s->after; };
-  if (!watched(a) || a == b) return b;
-  if (!watched(b)) return a;
-  const auto &front = a->first <= b->first ? a : b, &back = a->last >= b->last ? a : b;
-  auto s = std::make_shared<ExecStatus>();
-  s->before = front->before;
-  s->first = front->first;
-  s->after = back->after;
-  s->last = back->last;
-  return s;
+// What is known of `cache` when `rows` have been written to it. Executions in between that wrote neither do not count. Those that have ended
+// well are taken out when the list has become long, one query of an event for each, so that a step of a serving process pays for a few.
+std::shared_ptr<ExecStatus> status_with(const b200_buffer* cache, const b200_buffer* rows) {
+  constexpr int kMost = 16;
+  auto node = [](const ExecStatus& of, const std::shared_ptr<ReadyEvent>& landed, std::shared_ptr<ExecStatus> also) {
+    auto s = std::make_shared<ExecStatus>();
+    s->before = of.before;
+    s->after = of.after;
+    s->landed = landed;
+    s->length = also ? also->length + 1 : 1;
+    s->most = also ? also->most : kMost;
+    s->also = std::move(also);
+    return s;
+  };
+  std::shared_ptr<ExecStatus> now = cache->status;
+  if (!rows->status || !rows->status->watched()) return now;
+  if (now && now->after == rows->status->after) return now;
+  if (now && !now->landed) now = now->watched() ? node(*now, cache->ready, nullptr) : nullptr;      // of the execution that made the cache
+  now = node(*rows->status, rows->ready, std::move(now));
+  if (now->length <= now->most) return now;
+  std::vector<const ExecStatus*> kept;
+  for (const ExecStatus* s = now.get(); s; s = s->also.get()) {
+    if (cudaEventQuery(s->landed->ev) != cudaSuccess) { kept.push_back(s); continue; }
+    if (s->gave_up()) return node(*s, s->landed, nullptr);               // nothing makes that good again
+  }
+  std::shared_ptr<ExecStatus> list;
+  for (size_t k = kept.size(); k-- > 0;) list = node(*kept[k], kept[k]->landed, std::move(list));
+  if (list) list->most = std::max(kMost, 2 * list->length);
+  return list;
 }
 
 // In front of a change of `b` on the compute stream, and behind it.
@@ -3140,7 +3166,7 @@ b200_error* b200_cache_write_pages(b200_client* c, b200_buffer* cache, b200_buff
   int launches = 0;
   CUDA_TRY(launch_write_pages(shape, cache->ptr, rows->ptr, slots, (long long)n, c->compute, &launches));
   // an execution that gave up on a wait left its mark on the rows: what was made of them carries it too
-  cache->status = both_statuses(cache->status, rows->status);
+  cache->status = status_with(cache, rows);
   return after_change(c, cache, launches);
 } catch (const std::exception& e) {
   return make_error(B200_INTERNAL, std::string("write_pages: ") + e.what());

@@ -724,3 +724,36 @@ def test_window_attention_of_infinities_with_little_weight(client, dt, B, H, KH,
     fine = np.isfinite(raw)
     tol = attention_tolerance(want, mag, top, T, D, dt, 0.0 if dt == "f32" else U[dt])
     assert (np.abs(got - want)[fine] <= tol[fine]).all()
+
+
+@pytest.mark.parametrize("bad_rows", [False, True])
+@pytest.mark.parametrize("wait", [False, True])
+def test_a_cache_is_not_marked_by_others(client, bad_rows, wait):
+    """Among many executions whose rows go into a cache one gives up on a wait (test hook: a barrier nothing arrives at): the cache is invalid
+    if its rows went in, however long ago, and not if they did not."""
+    shape = (1, 2, 4, 1, 256)
+    cache = put(client, np.zeros((1, 2, 60, 4, 1, 256)), "bf16")
+    b = Builder()
+    x = b.arg((256, 256), "bf16")                                         # a product in 16 bits: its executions are watched
+    exe = client.compile(b.module([b.reshape(b.slice(b.dot_general(x, x, ([1], [0])), (0, 0), (8, 256)), shape)]))
+    arg = put(client, np.eye(256), "bf16")
+    client.synchronize()
+    for i in range(60):
+        if i == 7:
+            client.debug_arm_wait_expiry(1000)
+            bad = exe.execute([arg])[0]
+            if bad_rows:
+                client.write_pages(cache, bad, [28, 29, 30, 31])
+        rows = exe.execute([arg])[0]
+        client.write_pages(cache, rows, [4 * i, 4 * i + 1, 4 * i + 2, 4 * i + 3])
+        if wait:
+            rows.to_numpy()
+    if bad_rows:
+        for _ in range(2):
+            with pytest.raises(b200.B200Error, match="bounded"):
+                cache.to_numpy()
+    else:
+        got = cache.to_numpy()
+        assert np.array_equal(got[0], np.broadcast_to(np.eye(256, dtype=np.float32)[:8].reshape(2, 1, 4, 1, 256), (2, 60, 4, 1, 256)))
+    with pytest.raises(b200.B200Error):
+        client.synchronize()
