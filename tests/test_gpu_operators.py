@@ -757,3 +757,48 @@ def test_a_cache_is_not_marked_by_others(client, bad_rows, wait):
         assert np.array_equal(got[0], np.broadcast_to(np.eye(256, dtype=np.float32)[:8].reshape(2, 1, 4, 1, 256), (2, 60, 4, 1, 256)))
     with pytest.raises(b200.B200Error):
         client.synchronize()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("H", [1, 12])
+@pytest.mark.parametrize("n", [2, 300])
+def test_paged_attention_keeps_both_parts_of_a_weight(client, dt, H, n):
+    """Two positions whose contributions nearly cancel: what is left is what the rounding of a weight to 16 bits leaves of it."""
+    B, D, S = 40, 64, 16
+    less = rounded(np.linspace(0.1, 2.0, B), dt)                       # the second score lies this much below the first
+    pages = -(-n // S)
+    table, lengths = np.arange(B * pages, dtype=np.int32).reshape(B, pages), np.full(B, n, np.int32)
+    q, cache = np.zeros((B, H, D)), np.zeros((1, 2, B * pages, S, 1, D))
+    q[..., 0] = 1.0
+    cache[0, 0, ..., 0] = -100.0                                       # the others have no weight to speak of
+    for b in range(B):
+        for place, score, value in ((0, 0.0, rounded(np.exp(-less[b]), dt)), (1, -less[b], -1.0)):
+            cache[0, 0, table[b, place // S], place % S, 0, 0] = score
+            cache[0, 1, table[b, place // S], place % S] = value
+    got = run(client, lambda b, *a: b.paged_attention(*a, scale=1.0), [q, cache, table, lengths], [dt, dt, "i32", "i32"])[0]
+    want, mag, _ = operators.paged_attention(q, cache, table, lengths, scale=1.0, bounds=True)
+    # (the largest score that counts is 2)
+    tol = attention_tolerance(want, mag, 2.0, n, D, dt, U[dt] ** 2)
+    assert (np.abs(want) > 2 * tol).any()                              # a weight in one part, whose result is zero, would not pass
+    assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())
+
+
+def test_products_with_a_cache_behind_a_move(client):
+    """A product may read an argument ahead of its wait for the kernel in front of it; what a move writes is there all the same."""
+    D, S, P = 256, 64, 256
+    shape, n = (1, 2, P, S, 1, D), P * S
+    b = Builder()
+    x, c = b.arg((1, D), "bf16"), b.arg(shape, "bf16")
+    exe = client.compile(b.module([b.dot_general(x, c, ((1,), (5,)))]))
+    one = np.zeros((1, D))
+    one[0, 0] = 1.0
+    first, cache = put(client, one, "bf16"), put(client, np.zeros(shape), "bf16")
+    rows = [put(client, np.full((1, 2, n, 1, D), v), "bf16") for v in (1.0, 2.0)]
+    slots = np.arange(n, dtype=np.int32)[::-1].copy()
+    for _ in range(3):
+        outs = []
+        for i in range(20):
+            client.write_pages(cache, rows[i % 2], slots)
+            outs.append(exe.execute([first, cache])[0])
+        for i, o in enumerate(outs):
+            assert (o.to_numpy() == 1.0 + i % 2).all()

@@ -120,3 +120,59 @@ def test_serving_in_16_bits(client):
     want, got = (serve(c, "bf16", PROMPTS, 0) for c in (OracleClient(), client))
     for s in want:
         assert abs(want[s][1][0] - got[s][1][0]) < 0.1 * (1 + abs(want[s][1][0]))
+
+
+def forced(client, dtype, prompts, tokens, pages=24, page_size=4, ahead=0):
+    """Log probabilities of the best tokens and entropies of each step [steps + 1, prompts], with `tokens` [steps, prompts] given and not
+    chosen. `ahead`: tokens of sequences that come and go in front, so that the pages are others."""
+    def host(x):
+        return x.to_numpy() if hasattr(x, "to_numpy") else np.asarray(x)
+
+    W = [client.buffer_from_host(w, dtype="bf16" if dtype == "bf16" else None) for w in weights(dtype)]
+    B, T = len(prompts), max(len(p) for p in prompts)
+    padded, lengths = np.zeros((B, T), np.int32), np.array([len(p) for p in prompts], np.int32)
+    for row, p in zip(padded, prompts):
+        row[:len(p)] = p
+    kw = dict(SHAPE, dtype=dtype)
+    if isinstance(client, OracleClient):
+        client.shape = (SHAPE["layers"], 2, pages, page_size, 1, SHAPE["head_dim"])
+    cache = PagedCache(client, SHAPE["layers"], pages, page_size, 1, SHAPE["head_dim"], dtype)
+    seqs = [cache.add() for _ in prompts]
+    if ahead:
+        others = [cache.add() for _ in range(3)]
+        cache.extend(others, [ahead, 1, ahead])
+        cache.free(others[1])
+    prefill = client.compile(programs.gemma_paged_prefill(batch=B, prompt_len=T, **kw).text)
+    step = client.compile(programs.gemma_paged_step(batch=B, pages=pages, page_size=page_size, width=8, **kw).text)
+    _, lp, entropy, rows = prefill.execute(W + [client.buffer_from_host(padded), client.buffer_from_host(lengths)])
+    given, slots, at = cache.extend(seqs, lengths), np.full((B, T), -1, np.int32), 0
+    for b, n in enumerate(lengths):
+        slots[b, :n] = given[at:at + n]
+        at += n
+    cache.write(rows, slots.reshape(-1))
+    out = [(host(lp), host(entropy))]
+    for tok in tokens:
+        args = [client.buffer_from_host(a) for a in (np.asarray(tok, np.int32), cache.table(seqs, 8), cache.lengths(seqs))]
+        _, lp, entropy, rows = step.execute(W + [args[0], cache.buffer, *args[1:]])
+        cache.write(rows, cache.extend(seqs, [1] * B))
+        out.append((host(lp), host(entropy)))
+    return np.array(out, np.float64)
+
+
+@pytest.mark.gpu
+def test_steps_in_16_bits(client):
+    """bf16, prompts and eight steps with given tokens: the best tokens' log probabilities and the entropies, which change little where two
+    tokens change places, against the oracle on the same weights (within what test_serving_in_16_bits allows a log probability), and bit for
+    bit the same whichever pages the cache has."""
+    tokens = np.random.default_rng(5).integers(0, SHAPE["vocab"], (8, len(PROMPTS)))
+    want, got = (forced(c, "bf16", PROMPTS, tokens) for c in (OracleClient(), client))
+    assert want.shape == got.shape == (9, 2, len(PROMPTS))
+    assert (np.abs(want - got) < 0.1 * (1 + np.abs(want))).all()
+    np.testing.assert_array_equal(forced(client, "bf16", PROMPTS, tokens, pages=48, ahead=30), got)
+
+
+@pytest.mark.gpu
+def test_steps_in_32_bits(client):
+    tokens = np.random.default_rng(6).integers(0, SHAPE["vocab"], (8, len(PROMPTS)))
+    want, got = (forced(c, "f32", PROMPTS, tokens) for c in (OracleClient(), client))
+    np.testing.assert_allclose(got, want, rtol=1e-4, atol=1e-5)
