@@ -1741,6 +1741,7 @@ b200_error* run_plan(ExecCtx& x, const Plan& plan) {
                   " G=" + std::to_string(s.g16.G) + " a_kcontig=" + std::to_string(s.g16.a_ks == 1) + " b_kcontig=" +
                   std::to_string(s.g16.b_ks == 1) + " bn=" + std::to_string(s.g16.bn) + " splitK=" + std::to_string(s.g16.split_k);
           break;
+        case Step::OPERATOR: t.kind = "operator"; t.key = s.label; break;
         default: t.kind = "copy"; t.key = s.label; break;
       }
       cudaEventCreate(&t.a);

@@ -802,3 +802,19 @@ def test_products_with_a_cache_behind_a_move(client):
             outs.append(exe.execute([first, cache])[0])
         for i, o in enumerate(outs):
             assert (o.to_numpy() == 1.0 + i % 2).all()
+
+
+def test_profiles_name_operators(client):
+    """The report names an operator as one, with its own name, and its launches are not counted among copies."""
+    b = Builder()
+    x, t = b.arg((4, 1000), "f32"), b.arg((4,), "i32")
+    exe = client.compile(b.module(b.token_log_probs(x, t, top=3)))
+    args = [client.buffer_from_host(np.zeros((4, 1000), np.float32)), client.buffer_from_host(np.zeros(4, np.int32))]
+    client.set_profiling(True)
+    try:
+        exe.execute(args)
+        report = client.profile_report()
+    finally:
+        client.set_profiling(False)
+    kinds = {e["key"]: e["kind"] for e in report if "token_log_probs" in e["key"]}
+    assert set(kinds.values()) == {"operator"}, report
