@@ -818,3 +818,70 @@ def test_profiles_name_operators(client):
         client.set_profiling(False)
     kinds = {e["key"]: e["kind"] for e in report if "token_log_probs" in e["key"]}
     assert set(kinds.values()) == {"operator"}, report
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_operators_in_a_loop_of_unknown_length(client, dt):
+    """The first call goes round by the host, later ones on the device; other arguments, other lengths."""
+    rng = np.random.default_rng(3)
+    q, cache, table, lengths, _ = paged_case(rng, [300, 20], 4, 2, 64, 16, dt, False)
+    k, v = (rounded(rng.standard_normal((2, 40, 2, 64)), dt) for _ in range(2))
+    b = Builder()
+    a = [b.arg(q.shape, dt), b.arg(cache.shape, dt), b.arg(table.shape, "i32"), b.arg((2,), "i32"), b.arg((), "i32"), b.arg((2, 40, 4, 64), dt), b.arg(k.shape, dt), b.arg(k.shape, dt)]
+    outs = b.while_([b.const(0, "i32"), a[0], a[5]], lambda s, i, x, y: s.compare(i, a[4], "LT"),
+                    lambda s, i, x, y: [s.add(i, s.const(1, "i32")), s.paged_attention(x, a[1], a[2], a[3]), s.window_attention(y, a[6], a[7], a[3], window=9)])
+    exe = client.compile(b.module(list(outs[1:])))
+    prompts = rounded(rng.standard_normal((2, 40, 4, 64)), dt)
+    held = [put(client, x, d) for x, d in ((q, dt), (cache, dt), (table, "i32"), (lengths, "i32"))]
+    rest = [put(client, x, dt) for x in (prompts, k, v)]
+    seen = {}
+    for n in (3, 3, 1, 3, 2, 1, 2):
+        got = [o.to_numpy() for o in exe.execute([*held, client.buffer_from_host(np.array(n, np.int32)), *rest])]
+        if n in seen:
+            for g, w in zip(got, seen[n]):
+                np.testing.assert_array_equal(g, w)
+        seen[n] = got
+    want, mag, top = operators.paged_attention(q, cache, table, lengths, bounds=True)
+    assert (np.abs(seen[1][0] - want) <= attention_tolerance(want, mag, top, 300, 64, dt, 0.0 if dt == "f32" else U[dt])).all()
+    for n in (2, 3):                                               # each turn reads the last one's results as they are
+        want, mag, top = operators.paged_attention(seen[n - 1][0], cache, table, lengths, bounds=True)
+        assert (np.abs(seen[n][0] - want) <= attention_tolerance(want, mag, top, 300, 64, dt, 0.0 if dt == "f32" else U[dt])).all()
+        want, mag, top = operators.window_attention(seen[n - 1][1], k, v, lengths, window=9, bounds=True)
+        assert (np.abs(seen[n][1] - want) <= attention_tolerance(want, mag, top, 40, 64, dt, 0.0 if dt == "f32" else U[dt])).all()
+
+
+def test_two_clients_at_once():
+    """Two clients on two threads, with caches of their own. (A client is closed when nothing of it is left.)"""
+    import threading
+    errors = []
+
+    def use(c, seed):
+        rng = np.random.default_rng(seed)
+        q, cache, table, lengths, fresh = paged_case(rng, [500, 40, 7], 8, 2, 128, 16, "bf16", True)
+        x, y, z = prompt_case(rng, 1, 200, 2, 1, 64, "bf16")
+        for _ in range(10):
+            check_paged(c, q, cache, table, lengths, fresh, "bf16")
+        buf, rows = put(c, cache, "bf16"), rounded(rng.standard_normal((1, 2, 5, 2, 128)), "bf16")
+        for i in range(30):
+            slots, pairs = np.arange(5) + 5 * (i % 3), [(0, 5), (5, 0)]
+            c.write_pages(buf, put(c, rows, "bf16"), slots)
+            c.copy_pages(buf, pairs)
+            cache = operators.copy_pages(operators.write_pages(cache, rows, slots), pairs)
+        np.testing.assert_array_equal(buf.to_numpy(), cache)
+        check_prompt(c, x, y, z, None, "bf16")
+
+    def work(c, seed):
+        try:
+            use(c, seed)
+        except Exception as e:                  # handed to the test's thread
+            errors.append(repr(e))
+    clients = [b200.Client() for _ in range(2)]
+    threads = [threading.Thread(target=work, args=(c, k)) for k, c in enumerate(clients)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(timeout=120)
+    assert not errors and not any(t.is_alive() for t in threads), errors
+    for c in clients:
+        c.synchronize()
+        c.close()
