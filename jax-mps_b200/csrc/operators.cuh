@@ -36,11 +36,16 @@ cudaError_t launch_op(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, 
   return launch_kernel(cfg, kernel, std::forward<A>(args)...);
 }
 
-// More shared memory than 48 KB has to be asked for, once per kernel and device.
+// More shared memory than 48 KB has to be asked for, once per kernel and device. It counts as asked for behind the call and not in front of
+// it: another client's thread may be about to launch the same kernel.
 template <typename K>
 cudaError_t allow_smem(K* kernel, size_t bytes, bool (&done)[64]) {
-  if (!first_use_on_this_device(done)) return cudaSuccess;
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  int dev = 0;
+  const bool known = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
+  if (known && __atomic_load_n(&done[dev], __ATOMIC_ACQUIRE)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && known) __atomic_store_n(&done[dev], true, __ATOMIC_RELEASE);
+  return e;
 }
 
 __device__ __forceinline__ float to_float(float v) { return v; }
