@@ -105,7 +105,7 @@ class PagedCache:
         self.client.write_pages(self.buffer, rows, slots)
 
     def compact(self) -> int:
-        """Moves the pages in use to the lowest numbers; gives how many moved. Tables made before are void."""
+        """Moves the pages in use to the lowest numbers; gives how many moved. Tables and slots made before are void."""
         used = sorted({p for pages in self._pages.values() for p in pages})
         holes = [p for p in range(len(used)) if self._uses[p] == 0]
         moves = dict(zip([p for p in used if p >= len(used)], holes))

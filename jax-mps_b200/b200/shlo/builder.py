@@ -862,7 +862,7 @@ class Builder:
         """Causal attention of whole prompts: q [batch, tokens, heads, head_dim], k and v [batch, tokens, kv_heads, head_dim], and for
         a padded batch `lengths` i32[batch]; rows from a sequence's length on are zero and nobody sees them, nor does what a row does not see
         reach it, NaN and infinities included. `window`, `sinks` and
-        `scale` as in paged_attention. No gradient."""
+        `scale` as in paged_attention; 16-bit data has its weights rounded to 16 bits for the product with v. No gradient."""
         xs = [q, k, v] + ([lengths] if lengths is not None else [])
         config = {"scale": None if scale is None else float(scale), "window": window, "sinks": sinks}
         out = self._operator("window_attention", xs, [(q.shape, q.dtype)], config)

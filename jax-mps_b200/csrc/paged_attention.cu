@@ -149,7 +149,7 @@ struct Ring {
   static constexpr int ROW = DP * (int)sizeof(T), PIECES = ROW / 16;
   // Warps and the tiles that each has on its way or in use, by the bytes of a row: as many warps as registers let be, for a tile's products
   // are a chain (heads of 128, 32 sequences of up to 4096 positions, 16-bit: 8 warps an SM with three tiles 55.3 us, 12 with two 54.2; 32-bit
-  // heads of 64 58 and 46).
+  // heads of 64 58 and 46, which are 42 since).
   static constexpr int WARPS = ROW >= 768 ? 2 : ROW > 256 ? 6 : 4, STAGES = ROW >= 768 ? 3 : ROW > 128 ? 2 : 3;
   static constexpr int TILE = 16 * ROW, STAGE = 2 * TILE;            // bytes of the keys, of keys and values
   static constexpr int BYTES = WARPS * STAGES * STAGE;
