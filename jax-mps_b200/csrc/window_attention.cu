@@ -742,6 +742,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid
             const int part = ITEMS == 2 ? c / 2 : half;
             store32(t_s + C::weights(part), p);
             stored();
+            // A barrier's parity tells a phase from the next and not from the one after: who waits for the last tile's products below has
+            // to have seen those of the tile in front of it, and here the last ones cannot be through yet. (With one tile of queries, scores
+            // are issued in front of the last tile's products, so that having them says nothing of those, which wait for the slowest warp.)
+            if (c + 1 == PARTS && i > 0 && i + 1 == w.count) wait(PV_DONE + u, (j - 1) & 1);
             before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(P_FULL + 2 * place(u, j) + part));
@@ -749,6 +753,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid
         }
         const uint64_t all = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
         l += first(all) + second(all);
+        if (!ok) break;
       }
       if (!ok) break;
       if (w.count) {

@@ -885,3 +885,24 @@ def test_two_clients_at_once():
     for c in clients:
         c.synchronize()
         c.close()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("D,T", [(256, 300), (192, 257), (136, 200), (64, 300)])
+def test_window_attention_repeats_itself(client, dt, D, T):
+    """Several units of one tile of queries for each block (64 features: of two), tiles of keys whose products the slowest warp holds up: the same
+    bits from the first call of a program and from all others, in 180 heads of 30 sequences."""
+    rng = np.random.default_rng(D)
+    q, k, v = prompt_case(rng, 30, T, 6, 2, D, dt)
+    bufs = [put(client, x, dt) for x in (q, k, v)]
+    first = None
+    for window in (0, 0, 0, 150):
+        b = Builder()
+        exe = client.compile(b.module([b.window_attention(*[b.arg(x.shape, dt) for x in (q, k, v)], window=window)], name=f"jit_repeat_{window}"))
+        outs = [np.asarray(exe.execute(bufs)[0].to_numpy()) for _ in range(8)]
+        for o in outs[1:] + ([first] if first is not None and not window else []):
+            np.testing.assert_array_equal(o, outs[0])
+        first = outs[0] if first is None else first
+        for s in (0, 17):
+            want, mag, top = operators.window_attention(q[s:s + 1, :, ::5], k[s:s + 1], v[s:s + 1], window=window, bounds=True)
+            assert (np.abs(outs[0][s:s + 1, :, ::5] - want) <= attention_tolerance(want, mag, top, T, D, dt, U[dt])).all()
