@@ -585,6 +585,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NT>::WARPS * 32, Ring<T, DP, NT>::
       }
       if (count == 1) {
         const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        if (inv == 0.f) v = {0.f, 0.f, 0.f, 0.f};                   // no weight at all, whatever the values are
         T* to = (T*)a.out + ((long long)b * a.heads + h0 + h) * D + d;
         to[0] = from_float<T>(v.x * inv);
         to[1] = from_float<T>(v.y * inv);
@@ -608,8 +609,9 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   pdl_prologue();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = a.dim;
   auto part = [&](int first, int i, int h) { return a.parts + ((long long)(2 * (first + i) + (i == 0 ? 1 : 0)) * a.heads + h) * (D + 4); };
-  auto finish = [&](int pair, int d, const float4& v, float l) {
+  auto finish = [&](int pair, int d, float4 v, float l) {
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    if (inv == 0.f) v = {0.f, 0.f, 0.f, 0.f};
     T* to = (T*)a.out + (long long)pair * D + d;
     to[0] = from_float<T>(v.x * inv);
     to[1] = from_float<T>(v.y * inv);

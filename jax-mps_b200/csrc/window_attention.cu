@@ -766,8 +766,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) prompt_mma_kernel(const __grid
         if (!wait(PV_DONE + u, (it - 1) & 1)) break;
         after_sync();
       }
-      const bool some = w.count && row < w.n;
-      const float inv = some && (l > 0.f || l != l) ? 1.f / l : 0.f;
+      const bool some = w.count && row < w.n && (l > 0.f || l != l);      // whether the row has any weight to give
+      const float inv = some ? 1.f / l : 0.f;
       uint64_t odd = 0;                                              // NaN where one is not finite
 #pragma unroll
       for (int c0 = 0; c0 < (ITEMS == 2 ? DP : DP / 2); c0 += 32) {

@@ -906,3 +906,21 @@ def test_window_attention_repeats_itself(client, dt, D, T):
         for s in (0, 17):
             want, mag, top = operators.window_attention(q[s:s + 1, :, ::5], k[s:s + 1], v[s:s + 1], window=window, bounds=True)
             assert (np.abs(outs[0][s:s + 1, :, ::5] - want) <= attention_tolerance(want, mag, top, T, D, dt, U[dt])).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [1, 3, 300])
+def test_rows_whose_scores_are_all_minus_infinity(client, dt, n):
+    """They have no weight to give and are zero like rows that see nothing, whatever the values are."""
+    D = 64
+    q, k, v = np.ones((1, n, 2, D)), np.full((1, n, 1, D), -np.inf), np.ones((1, n, 1, D))
+    v[0, 0, 0, 3], v[0, n - 1, 0, 5], v[0, n // 2, 0, 7] = np.inf, np.nan, -np.inf
+    got = run(client, lambda b, q, k, v: b.window_attention(q, k, v), [q, k, v], [dt] * 3)[0]
+    with np.errstate(all="ignore"):
+        np.testing.assert_array_equal(got, operators.window_attention(q, k, v))
+    assert (got == 0).all()
+    pages = -(-n // 16)
+    cache = np.zeros((1, 2, pages, 16, 1, D))
+    cache[0].reshape(2, pages * 16, 1, D)[:, :n] = np.concatenate([k, v])
+    got = run(client, lambda b, *a: b.paged_attention(*a), [q[:, 0], cache, np.arange(pages, dtype=np.int32)[None], np.array([n], np.int32)], [dt, dt, "i32", "i32"])[0]
+    assert (got == 0).all()
