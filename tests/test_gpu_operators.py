@@ -924,3 +924,26 @@ def test_rows_whose_scores_are_all_minus_infinity(client, dt, n):
     cache[0].reshape(2, pages * 16, 1, D)[:, :n] = np.concatenate([k, v])
     got = run(client, lambda b, *a: b.paged_attention(*a), [q[:, 0], cache, np.arange(pages, dtype=np.int32)[None], np.array([n], np.int32)], [dt, dt, "i32", "i32"])[0]
     assert (got == 0).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_attention_of_values_that_are_nan_without_infinities(client, dt):
+    """NaN of values and keys reach what sees them and nothing else; there is nothing to make again."""
+    rng = np.random.default_rng(14)
+    q, cache, table, lengths, fresh = paged_case(rng, [700, 20, 300], 6, 2, 72, 16, dt, True)
+    cache[0, 1, table[0, 3], 5, 0, 9], cache[0, 1, table[0, 40], 1, 1] = np.nan, np.nan
+    cache[0, 0, table[1, 0], 7, 1, 3], fresh[1, 2, 0, 70] = np.nan, np.nan
+    got = run(client, lambda b, q, c, t, n, new: b.paged_attention(q, c, t, n, new=new), [q, cache, table, lengths, fresh], [dt, dt, "i32", "i32", dt])[0]
+    raw = operators.paged_attention(q, cache, table, lengths, fresh)
+    want, mag, top = operators.paged_attention(q, np.nan_to_num(cache), table, lengths, np.nan_to_num(fresh), bounds=True)
+    tol = attention_tolerance(want, mag, top, 701, 72, dt, 0.0 if dt == "f32" else U[dt] ** 2)
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(raw))
+    assert np.isnan(raw).any() and (np.abs(got - raw)[~np.isnan(raw)] <= tol[~np.isnan(raw)]).all()
+    q, k, v = prompt_case(rng, 2, 200, 6, 2, 72, dt)
+    v[0, 40, 0, 9], v[1, 0, 1], k[0, 150, 1, 3] = np.nan, np.nan, np.nan
+    got = run(client, lambda b, q, k, v: b.window_attention(q, k, v, window=70, sinks=2), [q, k, v], [dt] * 3)[0]
+    raw = operators.window_attention(q, k, v, window=70, sinks=2)
+    want, mag, top = operators.window_attention(q, np.nan_to_num(k), np.nan_to_num(v), window=70, sinks=2, bounds=True)
+    tol = attention_tolerance(want, mag, top, 200, 72, dt, 0.0 if dt == "f32" else U[dt])
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(raw))
+    assert (np.abs(got - want)[~np.isnan(raw)] <= tol[~np.isnan(raw)]).all()
