@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(Ring<T, DP, NT>::WARPS * 32, Ring<T, DP, NT>::
       }
     bool again = __any_sync(0xFFFFFFFFu, any_odd);
     if (again) {
-      // NaN that come of NaN are right as they are: only where the warp's values (32 bits: or keys) have an infinity, or a word that rounds to one,
+      // NaN that come of NaN are right as they are: only where the warp's values (32 bits: or keys or queries) have an infinity, or a word that rounds to one,
       // is there more to do.
       bool found = false;
 #pragma unroll 1
@@ -503,6 +503,8 @@ __global__ void __launch_bounds__(Ring<T, DP, NT>::WARPS * 32, Ring<T, DP, NT>::
                    infinite_word<T>(k.z) | infinite_word<T>(k.w);
         }
       }
+      if (WIDE)
+        for (int i = lane; i < nh * D; i += 32) found |= infinite_word<T>(((const uint32_t*)a.q)[((long long)b * a.heads + h0) * D + i]);
       again = __any_sync(0xFFFFFFFFu, found);
     }
     if (again) {

@@ -947,3 +947,22 @@ def test_attention_of_values_that_are_nan_without_infinities(client, dt):
     tol = attention_tolerance(want, mag, top, 200, 72, dt, 0.0 if dt == "f32" else U[dt])
     np.testing.assert_array_equal(np.isnan(got), np.isnan(raw))
     assert (np.abs(got - want)[~np.isnan(raw)] <= tol[~np.isnan(raw)]).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_attention_of_infinite_queries(client, dt):
+    """An infinite feature of a query makes scores of plus and minus infinity: of minus infinity alone, a row without weight; of both, none but
+    plus infinity's, which is no number."""
+    rng = np.random.default_rng(16)
+    q, cache, table, lengths, _ = paged_case(rng, [300, 40], 3, 1, 64, 16, dt, False)
+    cache[0, 0, ..., 5] = rounded(np.abs(cache[0, 0, ..., 5]) + 0.25, dt)
+    q[0, 0, 5], q[0, 2, 5], q[1, 1, 7] = -np.inf, np.inf, np.inf
+    got = run(client, lambda b, *a: b.paged_attention(*a), [q, cache, table, lengths], [dt, dt, "i32", "i32"])[0]
+    with np.errstate(all="ignore"):
+        raw = operators.paged_attention(q, cache, table, lengths)
+    assert (raw[0, 0] == 0).all() and np.isnan(raw[0, 2]).all() and np.isnan(raw[1, 1]).all()
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(raw))
+    want, mag, top = operators.paged_attention(np.where(np.isfinite(q), q, 0.0), cache, table, lengths, bounds=True)
+    fine = [(0, 1), (1, 0), (1, 2)]
+    tol = attention_tolerance(want, mag, top, 300, 64, dt, 0.0 if dt == "f32" else U[dt] ** 2)
+    assert (got[0, 0] == 0).all() and all((np.abs(got - want) <= tol)[i].all() for i in fine)
